@@ -119,6 +119,83 @@ void sh_cuda_add_layernorm(uint64_t h, uint64_t y, uint64_t a, uint64_t b, uint6
 int sh_cuda_attention_batched(uint64_t q, uint64_t k, uint64_t v, uint64_t o, uint32_t S, uint32_t D, uint32_t H,
                               uint32_t ldq, uint32_t ldk, uint32_t ldv, uint32_t ldo, float scale, uint32_t B);
 
+/* ---- decoding: paged 8-bit K / V cache and 4-bit weights ------------------------------------------------------------
+ * No counterpart in the reference (its attention reads whole fp16 K / V matrices, runtime/sh_ops.h:109-127, 277-304, and
+ * its GEMMs fp16 weights). One decode step of a batch of requests is
+ *     sh_cuda_gemv_w4 (Q|K|V) -> sh_rope -> sh_cuda_kv_tables -> sh_cuda_kv8_append -> sh_cuda_attention_kv8
+ *     -> sh_cuda_gemv_w4 (output projection), ...
+ * all on the library stream, with every length on the device, so that a step can be captured into a graph and replayed.
+ *
+ * The cache holds `pages` pages of `page` tokens. The codes of page p, head h, token t, column d are the bytes
+ *     k[p * page_stride + (h * page + t) * dh + d], v[the same]
+ * and stand for code * k_scale[p * heads + h] (v_scale for v): one fp32 scale, >= 0, per page and head.
+ *   fmt    SH_INT8 (two's complement) or SH_FP8 (e4m3: 4 exponent bits, bias 7; the NaN codes 0x7F, 0xFF stay unused)
+ *   page   16, 32, 64 or 128;  dh  64 or 128;  pages * page < 2^31
+ *   page_stride  bytes from page to page, a multiple of 16, >= heads * page * dh (more when K and V pages alternate in
+ *                one allocation)
+ *   k, v   16-byte aligned; k_scale, v_scale 4-byte aligned
+ * The struct is read during the call only. */
+typedef struct sh_cuda_kv8_t {
+    uint64_t k, v, k_scale, v_scale, page_stride;
+    uint32_t pages, page, heads, dh, fmt;
+} sh_cuda_kv8_t;
+
+/* Block tables and slot maps of one step from the requests' lengths. For R <= 8192 requests (int32 arrays on the
+ * device): lens[r] tokens are in the cache and add[r] follow in this step (0: none; < 0: the request has ended).
+ * table[r * ld_table + b] is the page of tokens [b page, (b + 1) page) of request r, ring[pages] the free pages in the
+ * order of their use: `count` entries from index `head` on, modulo pages, with pool = {head, count, ..}, eight words.
+ *   - A request that needs new pages takes them from the ring's head, requests in order. Requests whose blocks would
+ *     pass ld_table, and all from the first one on that the ring cannot serve whole, are put off: they keep their
+ *     length and get no slots (requests that need no new page are served all the same).
+ *   - A request that has ended gives its pages to the ring's tail (its table row is left as it was) and has length 0
+ *     afterwards; pages given back can be taken from the next call on.
+ * Writes: the new entries of table and ring; lens_out[R]; q_start[R + 1], the first row of each request's new tokens;
+ * for row i < t_cap slots[i] = page * (tokens per page) + offset and pos[i] = the token's position in its request (the
+ * row of a RoPE table), or slot -1 for the rows of put-off requests, and slot -1, pos 0 for rows past the last token;
+ * pool_out = {head, count, number of requests put off, ..}. lens_out may be lens and pool_out may be pool (a running
+ * pool); with other addresses a call can be repeated. Words 3..6 of pool_out are left alone, word 7 belongs to the
+ * library: zero before the first call. Returns 0 or -1 (reason printed). */
+int sh_cuda_kv_tables(uint64_t lens, uint64_t add, uint32_t R, uint32_t page, uint64_t table, uint32_t ld_table,
+                      uint64_t ring, uint32_t pages, uint64_t pool, uint64_t pool_out, uint64_t lens_out,
+                      uint64_t q_start, uint64_t slots, uint64_t pos, uint32_t t_cap);
+
+/* The rows k[T, heads * dh], v[T, heads * dh] (fp16, leading dims ldk, ldv) into the cache at slots[T] (int32; < 0: no
+ * row). Tokens of one page follow one another with rising slots, as sh_cuda_kv_tables lays them out; rows of a page
+ * before the first new one are its older tokens, rows after the last new one are left as they were. Per page and head
+ *     s' = max(s if there are older tokens, up8(max |x| / qmax)),  code = round(x / s'),  qmax = 127 or 448,
+ * rounding to nearest even, up8 = the next value with 8 significant bits (no quotient then lies within rounding error
+ * of a border between two codes without lying on it, so every correct division gives the same codes); when s' > s
+ * the older codes become round(code s / s'). +-infinity counts as +-65504, NaN as 0. A slot past the cache, or one
+ * that does not rise within its page, is not written and raises the device error word (2); a page whose tokens
+ * do not follow one another is left with unspecified codes. Returns 0, -1, or -3 for fmt. */
+int sh_cuda_kv8_append(const sh_cuda_kv8_t *cache, uint64_t k, uint64_t v, uint32_t T, uint32_t ldk, uint32_t ldv,
+                       uint64_t slots);
+
+/* Attention of the new rows of R requests over the cache: row q_start[r] + i of q (i < q_start[r + 1] - q_start[r] = n)
+ * is a query of request r, which has lens[r] tokens in the cache, these n last, and attends its tokens
+ * j <= lens[r] - n + i; query head h reads head h / (H / heads) of the cache. o = softmax(scale q k^T) v in the rows of q,
+ * fp16 (leading dims ldq, ldo); a row without any token gives zeros; rows of o outside [q_start[0], q_start[R]) and past T
+ * are left as they were. One token per request, a few drafted ones, and whole prompt chunks are all
+ * served, in any mixture. q holds T rows; max_q, the most rows of one request, only picks the kernel (a wrong value
+ * costs time). ws: ws_bytes >= SH_CUDA_KV8_WS_BYTES of device memory, 16-byte aligned, zeroed once before its first use,
+ * for the calls of one stream at a time (a graph that may run beside other calls has its own). A table entry outside the
+ * cache, or a length past ld_table * page, raises the device error word (2) and those tokens are left out. Returns 0,
+ * -1, or -3 for fmt. */
+#define SH_CUDA_KV8_WS_BYTES (48u << 20)
+int sh_cuda_attention_kv8(uint64_t q, uint64_t o, const sh_cuda_kv8_t *cache, uint64_t table, uint32_t ld_table,
+                          uint64_t lens, uint64_t q_start, uint32_t R, uint32_t T, uint32_t max_q, uint32_t H,
+                          uint32_t ldq, uint32_t ldo, float scale, uint64_t ws, size_t ws_bytes);
+
+/* Z[M, N] = epi(X[M, K] . W[K, N]) for 1 <= M <= 32 rows and 4-bit weights: row n of `codes` (ldw bytes, a multiple of 16,
+ * >= K / 2; 16-byte aligned) holds the codes of column n of W, k = 2 i in the low and k = 2 i + 1 in the high half of
+ * byte i, and W[k, n] = scales[n, k / group] * (code - zeros[n, k / group]): fp16 scales and uint8 zero points (0..15)
+ * of K / group columns, zeros == 0 meaning 8 everywhere. group 32, 64 or 128, K % group == 0. X, Z fp16 with leading
+ * dims ldx, ldz; fp32 accumulation in a fixed order. flags: SH_EPI_BIAS and SH_EPI_RESIDUAL as in sh_cuda_gemm (Z may be
+ * the residual, not X). Returns 0 or -1 (reason printed). */
+int sh_cuda_gemv_w4(uint64_t x, uint64_t codes, uint64_t scales, uint64_t zeros, uint64_t z, uint32_t M, uint32_t N,
+                    uint32_t K, uint32_t ldx, uint32_t ldw, uint32_t ldz, uint32_t group, uint64_t bias,
+                    uint64_t residual, uint32_t ldr, uint32_t flags);
+
 /* ---- synthetic inputs -------------------------------------------------------------------------------------------
  * N(mean, std) fp16 from the LCG of sh_test_fill_fp16: per element two draws d0, d1, u = (d + 0.5) / 2^24 and
  * Box-Muller z = sqrt(-2 ln u0) cos(2 pi u1), with ln and cos evaluated as fixed series of correctly rounded fp32

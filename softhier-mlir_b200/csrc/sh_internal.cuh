@@ -81,13 +81,16 @@ inline bool aligned16(uint64_t p) { return (p & 15u) == 0; }
 
 // Launch with programmatic stream serialisation: the kernel's set-up overlaps its predecessor's tail (the kernel
 // calls pdl_wait() before touching memory). SH_PDL=0 launches the plain way.
-template <typename... KArgs, typename... Args>
-cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
-                       Args &&...args) {
+inline bool pdl_enabled() {
     static const bool pdl = [] {
         const char *e = getenv("SH_PDL");
         return !(e && atoi(e) == 0);
     }();
+    return pdl;
+}
+template <typename... KArgs, typename... Args>
+cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                       Args &&...args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
@@ -97,7 +100,7 @@ cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t s
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = pdl ? 1 : 0;
+    cfg.numAttrs = pdl_enabled() ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 

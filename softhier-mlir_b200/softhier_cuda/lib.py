@@ -29,6 +29,15 @@ class GemmPlan(C.Structure):
     """sh_cuda_gemm_plan_t (include/sh_ops_cuda.h): the planner's choice for one GEMM shape."""
     _fields_ = [(n, u32) for n in ("kernel", "bn", "tiles_m", "tiles_n", "k_blocks", "splits", "full_units",
                                    "units", "grid")]
+
+
+class Kv8(C.Structure):
+    """sh_cuda_kv8_t (include/sh_ops_cuda.h): a paged 8-bit K / V cache."""
+    _fields_ = [(n, u64) for n in ("k", "v", "k_scale", "v_scale", "page_stride")] + \
+               [(n, u32) for n in ("pages", "page", "heads", "dh", "fmt")]
+
+
+KV8_P = C.POINTER(Kv8)
 FN_VOID = C.CFUNCTYPE(None)
 
 # name: (restype, [argtypes]) -- one entry per declaration in include/*.h
@@ -94,6 +103,10 @@ SIGNATURES: dict[str, tuple] = {
     "sh_cuda_scale_rows": (i32, [u64, u64, u32, u32, u32, u32, u64]),
     "sh_cuda_add_layernorm": (None, [u64, u64, u64, u64, u64, u64, u32, u32, u32, f32]),
     "sh_cuda_attention_batched": (i32, [u64, u64, u64, u64, u32, u32, u32, u32, u32, u32, u32, f32, u32]),
+    "sh_cuda_kv_tables": (i32, [u64, u64, u32, u32, u64, u32, u64, u32, u64, u64, u64, u64, u64, u64, u32]),
+    "sh_cuda_kv8_append": (i32, [KV8_P, u64, u64, u32, u32, u32, u64]),
+    "sh_cuda_attention_kv8": (i32, [u64, u64, KV8_P, u64, u32, u64, u64, u32, u32, u32, u32, u32, u32, f32, u64, sz]),
+    "sh_cuda_gemv_w4": (i32, [u64, u64, u64, u64, u64, u32, u32, u32, u32, u32, u32, u32, u64, u64, u32, u32]),
     "sh_cuda_fill_normal_fp16": (None, [u64, u32, u32, u32, u32, f32, f32]),
     "sh_cuda_host_fill_normal_fp16": (None, [vp, u32, u32, u32, u32, f32, f32]),
     "sh_cuda_gemm_splitk_noalloc": (i32, [u64, u64, u64, u32, u32, u32, u32, u32, u32, u64, u64, u32, u32, u32]),
@@ -108,6 +121,7 @@ EPI_ACCUMULATE, EPI_BIAS, EPI_GELU, EPI_RESIDUAL, GEMM_SIMT = 0x1, 0x2, 0x4, 0x8
 EPI_F32_OUT, EPI_ACC_F32_IN = 0x10, 0x20
 EPI_LN_IN, EPI_STATS_OUT = 0x40, 0x80
 SH_LLM_PAD = 0xFFFF
+KV8_WS_BYTES = 48 << 20
 SH_ALL = 0xFFFFFFFF
 SH_FP16, SH_FP8, SH_INT16, SH_INT8 = 0, 1, 2, 3
 SH_XM_AUTO, SH_XM_PANEL, SH_XM_WHOLE = 0, 1, 2
