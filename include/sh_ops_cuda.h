@@ -189,8 +189,8 @@ int sh_cuda_attention_kv8(uint64_t q, uint64_t o, const sh_cuda_kv8_t *cache, ui
 /* Z[M, N] = epi(X[M, K] . W[K, N]) for 1 <= M <= 32 rows and 4-bit weights: row n of `codes` (ldw bytes, a multiple of 16,
  * >= K / 2; 16-byte aligned) holds the codes of column n of W, k = 2 i in the low and k = 2 i + 1 in the high half of
  * byte i, and W[k, n] = scales[n, k / group] * (code - zeros[n, k / group]): fp16 scales and uint8 zero points (0..15)
- * of K / group columns, zeros == 0 meaning 8 everywhere. group 32, 64 or 128, K % group == 0. X, Z fp16 with leading
- * dims ldx, ldz; fp32 accumulation in a fixed order. flags: SH_EPI_BIAS and SH_EPI_RESIDUAL as in sh_cuda_gemm (Z may be
+ * of K / group columns, zeros == 0 meaning 8 everywhere. group 32, 64 or 128, K % group == 0, K <= 262144. X, Z fp16 with
+ * leading dims ldx, ldz; fp32 accumulation in a fixed order. flags: SH_EPI_BIAS and SH_EPI_RESIDUAL as in sh_cuda_gemm (Z may be
  * the residual, not X). Returns 0 or -1 (reason printed). */
 int sh_cuda_gemv_w4(uint64_t x, uint64_t codes, uint64_t scales, uint64_t zeros, uint64_t z, uint32_t M, uint32_t N,
                     uint32_t K, uint32_t ldx, uint32_t ldw, uint32_t ldz, uint32_t group, uint64_t bias,

@@ -89,7 +89,7 @@ def test_gemv_w4_refusals(lib, capfd):
     lib.sh_cuda_last_error()
     good = dict(x=A, codes=A, scales=A, zeros=0, z=A, M=4, N=64, K=256, ldx=256, ldw=128, ldz=64, group=64, bias=0, residual=0,
                 ldr=0, flags=0)
-    for kw in (dict(M=33), dict(group=16), dict(group=256), dict(K=224), dict(K=0), dict(ldx=255), dict(ldz=63), dict(ldw=112),
+    for kw in (dict(M=33), dict(group=16), dict(group=256), dict(K=224), dict(K=0), dict(K=(1 << 18) + 64, ldx=1 << 20, ldw=1 << 19), dict(ldx=255), dict(ldz=63), dict(ldw=112),
                dict(ldw=136), dict(x=0), dict(codes=0), dict(codes=A + 8), dict(scales=0), dict(z=0), dict(x=A + 1),
                dict(flags=L.EPI_BIAS), dict(flags=L.EPI_RESIDUAL), dict(flags=L.EPI_RESIDUAL, residual=A, ldr=63),
                dict(flags=L.EPI_GELU), dict(flags=L.EPI_ACCUMULATE)):

@@ -532,6 +532,13 @@ def test_w4_strides_and_odd_addresses(gpu_lib, M):
         _w4_case(gpu_lib, M, 96, 512, 64, True, L.EPI_RESIDUAL, ldx=ldx, ldz=ldz, ldw=ldw, offset=offset)
 
 
+@pytest.mark.parametrize("M,K,group", [(32, 8192, 64), (32, 28672, 128), (20, 65536, 32), (3, 1 << 18, 64), (1, 28672, 32),
+                                       (1, 1 << 18, 128), (2, 40960, 128)])
+def test_w4_deep(gpu_lib, M, K, group):
+    """X over several CTAs of a cluster, and in pieces of its rows where it does not fit beside them."""
+    _w4_case(gpu_lib, M, 70, K, group, True, L.EPI_BIAS | L.EPI_RESIDUAL)
+
+
 def test_w4_is_deterministic_and_exact_on_whole_numbers(gpu_lib):
     """Small whole numbers: every product and sum is exact, so each term is counted once and in its place."""
     rt, rng = gpu_lib, np.random.default_rng(5)
@@ -548,23 +555,58 @@ def test_w4_is_deterministic_and_exact_on_whole_numbers(gpu_lib):
         np.testing.assert_array_equal(_np(z).astype(np.float64), want)
 
 
-def test_w4_special_rows_stay_apart(gpu_lib):
-    """Infinity and NaN in one row of X reach that row of Z only."""
+@pytest.mark.parametrize("M", [2, 3, 6, 12])
+@pytest.mark.parametrize("N,K", [(64, 256), (40, 16384)])
+def test_w4_special_rows_stay_apart(gpu_lib, M, N, K):
+    """Infinity and NaN in one row of X reach that row of Z only, as IEEE sums have them."""
     rt = gpu_lib
-    x = torch.randn((3, 256), device=DEV).half()
-    codes = torch.randint(0, 256, (64, 128), device=DEV, dtype=torch.uint8)
-    scales = torch.full((64, 2), 0.01, dtype=torch.float16, device=DEV)
+    x = torch.randn((M, K), device=DEV).half()
+    codes = torch.randint(0, 256, (N, K // 2), device=DEV, dtype=torch.uint8)
+    scales = torch.full((N, K // 128), 0.01, dtype=torch.float16, device=DEV)
 
     def run(x):
-        z = torch.zeros((3, 64), dtype=torch.float16, device=DEV)
-        assert rt.lib.sh_cuda_gemv_w4(_p(x), _p(codes), _p(scales), 0, _p(z), 3, 64, 256, 256, 128, 64, 128, 0, 0, 0, 0) == 0
+        z = torch.zeros((M, N), dtype=torch.float16, device=DEV)
+        assert rt.lib.sh_cuda_gemv_w4(_p(x), _p(codes), _p(scales), 0, _p(z), M, N, K, K, K // 2, N, 128, 0, 0, 0, 0) == 0
         rt.check()
         return _np(z)
     good = run(x)
-    y = x.clone()
-    y[1, 17], y[1, 200] = float("nan"), float("inf")
-    got = run(y)
-    assert np.array_equal(got[[0, 2]], good[[0, 2]]) and not np.isfinite(got[1]).any()
+    rest = [i for i in range(M) if i != 1]
+    W = D.w4_weights(_np(codes), _np(scales), None, 128, K)
+    for specials in ({17: np.nan, 200: np.inf}, {K - 1: np.inf}, {5: -np.inf}, {5: np.inf, 9: np.inf}):
+        y = x.clone()
+        for k, v in specials.items():
+            y[1, k] = v
+        got = run(y)
+        assert np.array_equal(got[rest], good[rest])
+        with np.errstate(invalid="ignore"):
+            want = sum(W[k] * v for k, v in specials.items())          # inf, -inf, or NaN where a weight is 0
+        assert np.array_equal(np.isnan(got[1]), np.isnan(want))
+        ok = ~np.isnan(want)
+        assert np.array_equal(got[1][ok].astype(np.float64), want[ok])
+
+
+@pytest.mark.parametrize("M", [1, 2, 4])
+def test_w4_wide_range_of_x(gpu_lib, M):
+    """fp16 values from the smallest to the largest in one row: small ones beside weights that cancel or skip the large."""
+    rt, rng = gpu_lib, np.random.default_rng(7)
+    N, K, group = 90, 512, 64
+    codes = rng.integers(0, 256, (N, K // 2)).astype(np.uint8)
+    codes[::2, :64] = 0x88                              # zero weights below the large values
+    scales = rng.uniform(0.5, 1.5, (N, K // group)).astype(np.float16) * np.float16(2.0 ** -6)
+    x = np.ldexp(rng.standard_normal((M, K)), rng.integers(-24, 4, (M, K))).astype(np.float16)
+    x[:, :128] = np.where(rng.random((M, 128)) < 0.5, 65504.0, -65504.0)
+    x[:, 128:160] = 2.0 ** -24
+    d = [torch.from_numpy(a).to(DEV) for a in (x, codes, scales)]
+    z = torch.zeros((M, N), dtype=torch.float16, device=DEV)
+    assert rt.lib.sh_cuda_gemv_w4(_p(d[0]), _p(d[1]), _p(d[2]), 0, _p(z), M, N, K, K, K // 2, N, group, 0, 0, 0, 0) == 0
+    rt.check()
+    W = D.w4_weights(codes, scales, None, group, K)
+    want, mag = x.astype(np.float64) @ W, np.abs(x.astype(np.float64)) @ np.abs(W)
+    tol = 2.0 ** -11 * np.abs(want) + 2.0 ** -25 + (K + K // group + 16) * 2.0 ** -24 * mag
+    got = _np(z).astype(np.float64)
+    over = np.abs(want) >= 65520
+    assert np.all(np.isinf(got[np.abs(want) > 65600]))
+    assert (np.abs(got - want)[~over] <= tol[~over]).all()
 
 
 # ---- together ------------------------------------------------------------------------------------------------------------
