@@ -54,14 +54,20 @@ __device__ __forceinline__ uint32_t w4_fma(uint32_t a, uint32_t b, uint32_t c) {
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
     return r;
 }
+// (a & b) | c in one instruction (written in C, the two constants make it two)
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
 // codes 0 .. 7 of a word minus the zero point, as the pairs (0, 4), (1, 5), (2, 6), (3, 7)
 __device__ __forceinline__ void w4_word(uint32_t w, uint32_t zlo, uint32_t zhi, uint32_t (&h)[4]) {
     constexpr uint32_t kSixteenth = 0x2C002C00u;
     const uint32_t v = w >> 8;
-    h[0] = w4_sub((w & 0x000F000Fu) | 0x64006400u, zlo);
-    h[1] = w4_fma((w & 0x00F000F0u) | 0x64006400u, kSixteenth, zhi);
-    h[2] = w4_sub((v & 0x000F000Fu) | 0x64006400u, zlo);
-    h[3] = w4_fma((v & 0x00F000F0u) | 0x64006400u, kSixteenth, zhi);
+    h[0] = w4_sub(and_or(w, 0x000F000Fu, 0x64006400u), zlo);
+    h[1] = w4_fma(and_or(w, 0x00F000F0u, 0x64006400u), kSixteenth, zhi);
+    h[2] = w4_sub(and_or(v, 0x000F000Fu, 0x64006400u), zlo);
+    h[3] = w4_fma(and_or(v, 0x00F000F0u, 0x64006400u), kSixteenth, zhi);
 }
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar) {
