@@ -22,6 +22,7 @@ struct KvArgs {
     uint32_t ld_table, R, T, G, heads, pages, page_shift, ldq, ldo;
     float sl2;            // scale * log2(e)
     uint32_t vec;         // q rows take 16-byte loads, o rows 4-byte stores
+    uint32_t vec_o;       // o rows take 16-byte stores
     uint32_t *counters;   // arrivals per CTA whose last item goes on in others, zero between calls
     float *part;
     int *err;
@@ -589,6 +590,523 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
         for (int i = 0; i < kStages; ++i) drain_wait(full + i, phase ^ (i < (int)slot));
 }
 
+// ================================================================================================================
+// Many rows per request (prompt chunks): tcgen05. A CTA per SM walks its run of units (request, kv head, 256 rows, block of
+// 128 tokens; the blocks behind a tile's last row are left out). 512 threads:
+//   warp 0        copies: the pages' K and V boxes (8 bits) and scales into a ring of two blocks, as above
+//   warp 1        tcgen05.mma: per block and 128-row tile t  S_t = Q_t K^T (N = 128 tokens), then, when the softmax has
+//                 written P_t over S_t, O_t += P_t V with P_t read from tensor memory. The order P V of the block before, S of
+//                 this one, for one tile after the other keeps one tile's matrix products under the other's softmax.
+//   warps 4..7    turn a block's codes into fp16 operands in the swizzled layout of the matrix unit, once for both tiles
+//                 (one key row per lane: neither the reads nor the writes of a quarter-warp meet in a bank)
+//   warps 8..15   softmax, one row per thread (8..11 tile 0, 12..15 tile 1), the scores read from tensor memory twice, for
+//                 the maximum and for the weights, so that 512 threads fit the register file
+// The scales of 16 tokens are one multiply-add per score (x = ks s + log2 vs) and one per 16 weights. A block is 2048 cycles of
+// tensor work and as many of the special-function unit's (32768 exponentials).
+// ================================================================================================================
+constexpr uint32_t kTlRows = 128, kTlKeys = 128, kTlItem = 256, kTlThreads = 512, kTlStages = 2;
+
+template <int DH>
+struct TilesSmem {
+    static constexpr uint32_t kChunk = 128 * 128;                      // 128 rows x 64 fp16 columns
+    static constexpr uint32_t kTile = DH / 64 * kChunk, kBox = 16 * DH, kCodes = kTlKeys * DH;
+    static constexpr uint32_t kQ = 0, kK = kQ + 2 * kTile, kV = kK + kTile, kRing = kV + kTile;
+    static constexpr uint32_t kInfo = kRing + kTlStages * 2 * kCodes;  // [stages][8] {ks, vs, usable}
+    static constexpr uint32_t kGroup = kInfo + kTlStages * 128;        // [2][8] {ks scale log2 e, log2 vs, 1 / vs}
+    static constexpr uint32_t kBars = kGroup + 256, kMisc = kBars + 32 * 8, kBytes = kMisc + 256 + 1024;
+};
+
+// A tile of a request in the run of a CTA
+struct TileCursor {
+    uint32_t r, kvh, tile, tiles, b, blocks;
+    ReqView v;
+    uint32_t row0, nrows;
+    int lim_hi;
+};
+__device__ __forceinline__ void tile_sizes(TileCursor &k, const KvArgs &a) {      // after tile or request changed
+    k.row0 = k.tile * kTlItem, k.nrows = min(kTlItem, k.v.nq * a.G - k.row0);
+    k.lim_hi = min(max(k.v.base + (int)((k.row0 + k.nrows - 1) / a.G) + 1, 0), (int)k.v.ctx);
+    k.blocks = max(1u, (uint32_t)(k.lim_hi + (int)kTlKeys - 1) / kTlKeys);
+}
+__device__ __forceinline__ void tile_request(TileCursor &k, const KvArgs &a) {
+    k.v = req_view(a, k.r);
+    k.tiles = (k.v.nq * a.G + kTlItem - 1) / kTlItem;
+}
+__device__ __forceinline__ void tile_next(TileCursor &k, const KvArgs &a) {       // the next tile's first block
+    k.b = 0;
+    if (++k.tile == k.tiles) {
+        k.tile = 0;
+        if (++k.kvh == a.heads) {
+            k.kvh = 0;
+            do {
+                if (++k.r >= a.R) return;
+                tile_request(k, a);
+            } while (k.tiles == 0);
+        }
+    }
+    tile_sizes(k, a);
+}
+
+template <int DH, bool FP8>
+__global__ void __launch_bounds__(kTlThreads, 1)
+    k_attn_kv8_tiles(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, KvArgs a) {
+    using SM = TilesSmem<DH>;
+    typedef unsigned long long u64;
+    constexpr uint32_t kTmS = 0, kTmO = 2 * kTlKeys;                   // tensor memory: S_t / P_t, O_t
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(sm + SM::kBars);
+    uint64_t *c_full = bars, *c_empty = bars + 2;                      // ring of codes
+    uint64_t *k_full = bars + 4, *k_empty = bars + 5, *v_full = bars + 6, *v_empty = bars + 7;
+    uint64_t *q_full = bars + 8, *s_full = bars + 10, *p_full = bars + 12, *o_full = bars + 14, *mdone = bars + 16;
+    struct Misc {
+        u64 part[kTlThreads / 32];
+        u64 off;
+        uint32_t r, flag, tmem;
+        int abort;
+    };
+    Misc &mi = *reinterpret_cast<Misc *>(sm + SM::kMisc);
+    volatile int *abort = &mi.abort;
+    const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const uint32_t page1 = (1u << a.page_shift) - 1;
+    if (t == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(c_full + i, 1 + 8), mbar_init(c_empty + i, 4);
+            mbar_init(q_full + i, 4), mbar_init(s_full + i, 1), mbar_init(p_full + i, 4), mbar_init(o_full + i, 1);
+        }
+        mbar_init(k_full, 4), mbar_init(k_empty, 1), mbar_init(v_full, 4), mbar_init(v_empty, 1), mbar_init(mdone, 1);
+        mi.abort = 0;
+        prefetch_tmap(&mk), prefetch_tmap(&mv);
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(&mi.tmem, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = mi.tmem;
+    pdl_launch_dependents();
+    pdl_wait();
+
+    // ---- this CTA's run of units ------------------------------------------------------------------------------------
+    auto request_units = [&](uint32_t r, u64 stop, u64 &off) -> u64 {      // units of one head; stops in the tile that holds `stop`
+        TileCursor k;
+        k.r = r;
+        tile_request(k, a);
+        u64 n = 0;
+        for (k.tile = 0; k.tile < k.tiles; ++k.tile) {
+            tile_sizes(k, a);
+            if (n + k.blocks > stop) {
+                off = n;
+                return k.tile;
+            }
+            n += k.blocks;
+        }
+        return n;
+    };
+    const uint32_t per_t = (a.R + kTlThreads - 1) / kTlThreads, r0 = min(t * per_t, a.R), r1 = min(r0 + per_t, a.R);
+    u64 sum = 0, none;
+    for (uint32_t r = r0; r < r1; ++r) {
+        sum += a.heads * request_units(r, ~0ull, none);
+        if (blockIdx.x == 0 && a.lens[r] > (int)(a.ld_table << a.page_shift)) atomicCAS(a.err, 0, (int)sh::kErrBadArgs);
+    }
+    u64 incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 x = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= (uint32_t)o) incl += x;
+    }
+    if (lane == 31) mi.part[warp] = incl;
+    __syncthreads();
+    u64 total = 0;
+    for (uint32_t w = 0; w < kTlThreads / 32; ++w) {
+        if (w < warp) incl += mi.part[w];
+        total += mi.part[w];
+    }
+    const u64 per = (total + gridDim.x - 1) / gridDim.x, begin = per * blockIdx.x, end = min(total, begin + per);
+    if (begin < end && begin >= incl - sum && begin < incl) {
+        u64 off = begin - (incl - sum);
+        for (uint32_t r = r0; r < r1; ++r) {
+            const u64 n = a.heads * request_units(r, ~0ull, none);
+            if (off < n) {
+                mi.r = r, mi.off = off;
+                break;
+            }
+            off -= n;
+        }
+    }
+    __syncthreads();
+    TileCursor k0 = {};
+    if (begin < end) {
+        k0.r = mi.r;
+        const u64 one = request_units(k0.r, ~0ull, none);
+        k0.kvh = (uint32_t)(mi.off / one);
+        u64 before = 0;
+        const u64 in = mi.off - k0.kvh * one;
+        k0.tile = (uint32_t)request_units(k0.r, in, before);
+        tile_request(k0, a);
+        tile_sizes(k0, a);
+        k0.b = (uint32_t)(in - before);
+    }
+
+    if (warp == 0) {
+        // ---------------- copies: lane i has tokens 16 i .. of a block ----------------
+        TileCursor k = k0;
+        uint32_t st = 0, ph = 0, n = 0;
+        auto lookup = [&]() {
+            const uint32_t tok = k.b * kTlKeys + lane * 16;
+            return lane < 8 && (int)tok < k.lim_hi ? a.table[(size_t)k.r * a.ld_table + (tok >> a.page_shift)] : -1;
+        };
+        int id = begin < end ? lookup() : -1;
+        for (u64 u = begin; u < end; ++u, ++n) {
+            const uint32_t tok = k.b * kTlKeys + lane * 16;
+            const bool used = lane < 8 && (int)tok < k.lim_hi, ok = used && (uint32_t)id < a.pages;
+            const int row = (int)((k.kvh << a.page_shift) + (tok & page1)), page = id;
+            const size_t at = (size_t)(uint32_t)id * a.heads + k.kvh;
+            if (u + 1 < end) {
+                if (++k.b == k.blocks) tile_next(k, a);
+                id = lookup();
+            }
+            if (n >= kTlStages) mbar_wait(c_empty + st, ph ^ 1u, abort, a.err);
+            uint64_t *bar = c_full + st;
+            const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, ok));
+            if (lane == 0) mbar_arrive_expect_tx(bar, boxes * 2 * SM::kBox);
+            __syncwarp();
+            if (lane < 8) {
+                float *info = reinterpret_cast<float *>(sm + SM::kInfo + (st * 8 + lane) * 16);
+                info[2] = ok;
+                if (ok) {
+                    uint8_t *dst = sm + SM::kRing + st * 2 * SM::kCodes + lane * SM::kBox;
+                    tma_load_3d(dst, &mk, bar, 0, row, page);
+                    tma_load_3d(dst + SM::kCodes, &mv, bar, 0, row, page);
+                    cp_async4(smem_u32(info), a.ks + at);
+                    cp_async4(smem_u32(info) + 4, a.vs + at);
+                } else if (used) {
+                    atomicCAS(a.err, 0, (int)sh::kErrBadArgs);
+                }
+                cp_async_arrive(bar);
+            }
+            if (++st == kTlStages) st = 0, ph ^= 1u;
+        }
+        // every copy has landed before the CTA may exit
+        for (uint32_t i = 0; i < min(n, kTlStages); ++i) {
+            const uint32_t last = n - 1 - i;
+            if (lane == 0) drain_wait(c_full + last % kTlStages, last / kTlStages & 1);
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issue: the whole warp walks the loop, lane 0 issues ----------------
+        const uint32_t is0 = lane == 0 ? 1u : 0u;
+        constexpr uint32_t idesc_s = umma_idesc_f16(kTlRows, kTlKeys, 0, 0), idesc_o = umma_idesc_f16(kTlRows, DH, 0, 1);
+        const uint64_t qd = sw128_desc(smem_u32(sm + SM::kQ), 16, 1024), kd = sw128_desc(smem_u32(sm + SM::kK), 16, 1024);
+        const uint64_t vd = sw128_desc(smem_u32(sm + SM::kV), SM::kChunk, 1024);
+        uint32_t kn = 0, vn = 0, pn[2] = {0, 0}, qn[2] = {0, 0};      // phases seen of each barrier
+        TileCursor k = k0;
+        for (u64 u = begin; u < end;) {
+            const uint32_t nb = (uint32_t)min((u64)(k.blocks - k.b), end - u), nt = k.nrows > kTlRows ? 2u : 1u;
+            // step j: P V of block j - 1, S of block j
+            for (uint32_t j = 0; j <= nb; ++j) {
+                if (j > 0) mbar_wait(v_full, vn++ & 1u, abort, a.err);
+                if (j < nb) mbar_wait(k_full, kn++ & 1u, abort, a.err);
+#pragma unroll 1
+                for (uint32_t t2 = 0; t2 < nt; ++t2) {
+                    if (j > 0) {
+                        mbar_wait(p_full + t2, pn[t2]++ & 1u, abort, a.err);
+                        tc_fence_after();
+#pragma unroll
+                        for (int i = 0; i < (int)kTlKeys / 16; ++i)
+                            umma_f16_ts_if(is0, tmem + kTmO + t2 * DH, tmem + kTmS + t2 * kTlKeys + i * 8,
+                                           vd + (uint64_t)(i * (2048 >> 4)), idesc_o, (j == 1 && i == 0) ? 0u : 1u);
+                        if (j == nb) umma_commit_if(is0, o_full + t2);
+                    }
+                    if (j < nb) {
+                        if (j == 0) mbar_wait(q_full + t2, qn[t2]++ & 1u, abort, a.err);
+                        tc_fence_after();
+#pragma unroll
+                        for (int i = 0; i < DH / 16; ++i) {
+                            const uint32_t at = ((uint32_t)(i / 4) * SM::kChunk + (i % 4) * 32) >> 4;
+                            umma_f16_ss_if(is0, tmem + kTmS + t2 * kTlKeys, qd + (t2 * SM::kTile >> 4) + at, kd + at, idesc_s,
+                                           i > 0 ? 1u : 0u);
+                        }
+                        umma_commit_if(is0, s_full + t2);
+                    }
+                }
+                if (j > 0) umma_commit_if(is0, v_empty);
+                if (j < nb) umma_commit_if(is0, k_empty);
+            }
+            u += nb;
+            if (u < end) tile_next(k, a);
+        }
+        // tensor memory may only be freed once every issued MMA has completed
+        umma_commit_if(is0, mdone);
+        if (is0) drain_wait(mdone, 0);
+    } else if (warp >= 4 && warp < 8) {
+        // ---------------- codes -> fp16: lane has key row 32 (warp - 4) + lane ----------------
+        const uint32_t row = (warp - 4) * 32 + lane, grp = row >> 4;
+        uint32_t st = 0, ph = 0, n = 0;
+        TileCursor k = k0;
+        auto convert = [&](const uint8_t *src, uint8_t *dst, bool keep) {
+#pragma unroll
+            for (int p = 0; p < DH / 16; ++p) {
+                // 16 codes: piece p of the row in the ring's swizzle; 32 bytes of fp16: pieces 2 p, 2 p + 1 of the 64-column chunk
+                const uint32_t pos = DH == 128 ? (p ^ (row & 7)) : (p ^ (row >> 1 & 3));
+                const uint4 x = lds16(smem_u32(src) + row * DH + pos * 16);
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                uint32_t h[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (FP8) {
+                        h[2 * i] = e4m3x2_to_h2(w[i] & 0xFFFFu), h[2 * i + 1] = e4m3x2_to_h2(w[i] >> 16);
+                    } else {
+                        const uint32_t y = w[i] ^ 0x80808080u;
+                        h[2 * i] = hsub2(__byte_perm(y, 0x64646464u, 0x4140), kMagicVal);
+                        h[2 * i + 1] = hsub2(__byte_perm(y, 0x64646464u, 0x4342), kMagicVal);
+                    }
+                }
+                if (!keep)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) h[i] = 0;
+                uint8_t *to = dst + (p >> 2) * SM::kChunk + row * 128;
+                const uint32_t piece = (p & 3) * 2;
+                *reinterpret_cast<uint4 *>(to + ((piece ^ (row & 7)) * 16)) = make_uint4(h[0], h[1], h[2], h[3]);
+                *reinterpret_cast<uint4 *>(to + (((piece + 1) ^ (row & 7)) * 16)) = make_uint4(h[4], h[5], h[6], h[7]);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+        };
+        for (u64 u = begin; u < end; ++u, ++n) {
+            mbar_wait(c_full + st, ph, abort, a.err);
+            const float4 info = *reinterpret_cast<const float4 *>(sm + SM::kInfo + (st * 8 + grp) * 16);
+            const bool ok = info.z != 0.f;
+            const uint8_t *codes = sm + SM::kRing + st * 2 * SM::kCodes;
+            if (n > 0) mbar_wait(k_empty, (n - 1) & 1u, abort, a.err);
+            if ((lane & 15) == 0) {
+                const float vs = ok ? fmaxf(info.y, 0x1p-80f) : 1.f;
+                *reinterpret_cast<float4 *>(sm + SM::kGroup + ((n & 1) * 8 + grp) * 16) =
+                    make_float4(ok ? info.x * a.sl2 : 0.f, ok ? __log2f(vs) : -INFINITY, __frcp_rn(vs), 0.f);
+            }
+            convert(codes, sm + SM::kK, ok);
+            if (lane == 0) mbar_arrive(k_full);
+            if (n > 0) mbar_wait(v_empty, (n - 1) & 1u, abort, a.err);
+            // rows that are no keys can hold anything; their weights are 0
+            convert(codes + SM::kCodes, sm + SM::kV, ok && (int)(k.b * kTlKeys + row) < k.lim_hi);
+            if (lane == 0) mbar_arrive(v_full), mbar_arrive(c_empty + st);
+            if (++st == kTlStages) st = 0, ph ^= 1u;
+            if (u + 1 < end && ++k.b == k.blocks) tile_next(k, a);
+        }
+    } else if (warp >= 8) {
+        // ---------------- softmax and output ----------------
+        const uint32_t t2 = (warp - 8) >> 2, quarter = warp & 3, row = quarter * 32 + lane;      // row of the tile
+        const uint32_t st = t - 256;                                                              // of 256 softmax threads
+        const uint32_t lane_base = tmem + (quarter * 32u << 16);
+        const uint32_t s_addr = lane_base + kTmS + t2 * kTlKeys, o_addr = lane_base + kTmO + t2 * DH;
+        uint32_t n = 0, sn = 0, on = 0;      // blocks of the run, blocks of this tile, items of this tile
+        TileCursor k = k0;
+        auto group_sync = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+        for (u64 u = begin; u < end;) {
+            const uint32_t b0 = k.b, nb = (uint32_t)min((u64)(k.blocks - k.b), end - u), rr = t2 * kTlRows + row;
+            const bool live = k.nrows > t2 * kTlRows, mine = rr < k.nrows;      // the tile's, this row's
+            const uint32_t qi = (k.row0 + rr) / a.G, gi = (k.row0 + rr) - qi * a.G;
+            const int ctx = (int)k.v.ctx;
+            const int lim = mine ? min(max(k.v.base + (int)qi + 1, 0), ctx) : k.lim_hi;
+            const int lim_lo = min(max(k.v.base + (int)((k.row0 + t2 * kTlRows) / a.G) + 1, 0), ctx);
+            float m = -INFINITY, l = 0.f;
+            if (live) {
+                // Q row -> swizzled operand (the tile's score products of the item before have completed)
+                const __half *qp = a.q + (size_t)(k.v.qs + qi) * a.ldq + ((size_t)k.kvh * a.G + gi) * DH;
+                uint8_t *to = sm + SM::kQ + t2 * SM::kTile + row * 128;
+#pragma unroll 4
+                for (int p = 0; p < DH / 8; ++p) {
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (mine) {
+                        if (a.vec) {
+                            x = *reinterpret_cast<const uint4 *>(qp + p * 8);
+                        } else {
+                            uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) w[e >> 1] |= (uint32_t)__half_as_ushort(qp[p * 8 + e]) << (16 * (e & 1));
+                            x = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    }
+                    *reinterpret_cast<uint4 *>(to + (p >> 3) * SM::kChunk + (((p & 7) ^ (row & 7)) * 16)) = x;
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_full + t2);
+            }
+            for (uint32_t j = 0; j < nb; ++j, ++n) {
+                if (!live) continue;
+                const int key0 = (int)((b0 + j) * kTlKeys);
+                const float4 *grp = reinterpret_cast<const float4 *>(sm + SM::kGroup + (n & 1) * 128);
+                mbar_wait(s_full + t2, sn++ & 1u, abort, a.err);      // and P V of the block before is complete
+                tc_fence_after();
+                const bool edge = key0 + (int)kTlKeys > lim_lo;
+                // exponents of 32 keys: x = s ks scale log2 e + log2 vs
+                auto exponents = [&](const uint32_t (&v)[32], float (&x)[32], int c) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float4 gr = grp[2 * c + h];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[16 * h + i] = fmaf(__uint_as_float(v[16 * h + i]), gr.x, gr.y);
+                    }
+                    if (edge) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (key0 + 32 * c + i >= lim) x[i] = -INFINITY;
+                    }
+                };
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t v[32];
+                    float x[32];
+                    tmem_ld_32x32b_x32(s_addr + 32 * c, v);
+                    tmem_ld_wait();
+                    exponents(v, x, c);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], x[i]);
+                }
+                const float mb = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                // the maximum only moves when a weight would pass 2^8 (exact room in fp16); O is rescaled then
+                float alpha = 1.f;
+                const bool raise = mb > m + 8.f;
+                if (raise) {
+                    alpha = fast_exp2(m - mb);
+                    l *= alpha;
+                    m = mb;
+                }
+                if (j > 0 && __any_sync(0xffffffffu, raise)) {
+#pragma unroll 1
+                    for (int c = 0; c < DH / 32; ++c) {
+                        uint32_t v[32];
+                        tmem_ld_32x32b_x32(o_addr + c * 32, v);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+                        tmem_st_32x32b_x32(o_addr + c * 32, v);
+                    }
+                }
+                const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t v[32], packed[16];
+                    float x[32];
+                    tmem_ld_32x32b_x32(s_addr + 32 * c, v);
+                    tmem_ld_wait();
+                    exponents(v, x, c);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float p0 = fast_exp2(x[16 * h + 2 * i] - ms), p1 = fast_exp2(x[16 * h + 2 * i + 1] - ms);
+                            s4[(2 * i) & 3] += p0, s4[(2 * i + 1) & 3] += p1;
+                            packed[8 * h + i] = pack_h2(p0, p1);
+                        }
+                        l = fmaf((s4[0] + s4[1]) + (s4[2] + s4[3]), grp[2 * c + h].z, l);
+                    }
+                    tmem_st_32x32b_x16(s_addr + 16 * c, packed);      // over scores that have been read
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + t2);
+            }
+            // ---- the item's end: O / l, or partial sums of an item that other CTAs share ----
+            if (live) {
+                mbar_wait(o_full + t2, on++ & 1u, abort, a.err);
+                tc_fence_after();
+            }
+            const bool whole = b0 == 0 && nb == k.blocks;
+            const uint32_t slot = 2 * blockIdx.x + (b0 == 0 ? 1 : 0);
+            constexpr size_t kSlot = (size_t)kTlItem * (DH + 2);
+            float *po = a.part + slot * kSlot, *pm = po + kTlItem * DH, *pl = pm + kTlItem;      // [DH][256], [256], [256]
+            __half *op = a.o + (size_t)(k.v.qs + qi) * a.ldo + ((size_t)k.kvh * a.G + gi) * DH;
+            auto write_out = [&](const float (&y)[32], int c, float inv) {
+                if (a.vec_o) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<uint4 *>(op + c * 32 + q * 8) =
+                            make_uint4(pack_h2(y[8 * q] * inv, y[8 * q + 1] * inv), pack_h2(y[8 * q + 2] * inv, y[8 * q + 3] * inv),
+                                       pack_h2(y[8 * q + 4] * inv, y[8 * q + 5] * inv),
+                                       pack_h2(y[8 * q + 6] * inv, y[8 * q + 7] * inv));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) op[c * 32 + i] = __float2half_rn(y[i] * inv);
+                }
+            };
+            if (live) {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+                for (int c = 0; c < DH / 32; ++c) {
+                    uint32_t v[32];
+                    float y[32];
+                    tmem_ld_32x32b_x32(o_addr + c * 32, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(v[i]);
+                    if (mine) {
+                        if (whole) {
+                            write_out(y, c, inv);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) po[(size_t)(c * 32 + i) * kTlItem + rr] = y[i];
+                        }
+                    }
+                }
+                tc_fence_before();
+                if (mine && !whole) pm[rr] = m, pl[rr] = l;
+            }
+            if (!whole) {
+                const u64 i0 = u - b0;      // the item's first unit: its CTA counts the arrivals
+                const uint32_t c0 = (uint32_t)(i0 / per), c1 = (uint32_t)((i0 + k.blocks - 1) / per);
+                group_sync();
+                if (st == 0) {
+                    const uint32_t before = atom_add_acq_rel_gpu(a.counters + c0, 1u);
+                    mi.flag = before == c1 - c0;
+                    if (mi.flag) a.counters[c0] = 0;      // for the next call
+                }
+                group_sync();
+                if (mi.flag && mine) {
+                    const uint32_t parts = c1 - c0 + 1;
+                    auto part = [&](uint32_t i) { return a.part + (size_t)(2 * (c0 + i) + (i == 0)) * kSlot; };
+                    float mt = -INFINITY, lt = 0.f;
+                    for (uint32_t i = 0; i < parts; ++i) mt = fmaxf(mt, __ldcg(part(i) + kTlItem * DH + rr));
+                    for (uint32_t i = 0; i < parts; ++i) {
+                        const float mi2 = __ldcg(part(i) + kTlItem * DH + rr);
+                        if (mi2 != -INFINITY) lt = fmaf(__ldcg(part(i) + kTlItem * DH + kTlItem + rr), fast_exp2(mi2 - mt), lt);
+                    }
+                    const float inv = lt == 0.f ? 0.f : 1.f / lt;
+#pragma unroll 1
+                    for (int c = 0; c < DH / 32; ++c) {
+                        float y[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) y[i] = 0.f;
+                        for (uint32_t p = 0; p < parts; ++p) {
+                            const float mp = __ldcg(part(p) + kTlItem * DH + rr);
+                            const float f = mp == -INFINITY ? 0.f : fast_exp2(mp - mt);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                y[i] = fmaf(__ldcg(part(p) + (size_t)(c * 32 + i) * kTlItem + rr), f, y[i]);
+                        }
+                        write_out(y, c, inv);
+                    }
+                }
+            }
+            u += nb;
+            if (u < end) tile_next(k, a);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
 constexpr size_t kCounterBytes = 16384;
 constexpr uint32_t kMaxSms = 160;         // the grid is cut there, so that the workspace is
 
@@ -603,6 +1121,16 @@ cudaError_t launch_rows(KvArgs &a, const CUtensorMap &mk, const CUtensorMap &mv,
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSmem<DH, NT, NW>::kBytes);
     if (e != cudaSuccess) return e;
     return sh::launch_pdl(kernel, dim3(sms * kPerSm), dim3(NW * 32), RowsSmem<DH, NT, NW>::kBytes, st, mk, mv, a);
+}
+
+template <int DH, bool FP8>
+cudaError_t launch_tiles(KvArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int sms, cudaStream_t st) {
+    static_assert(kCounterBytes + (size_t)2 * kMaxSms * kTlItem * (DH + 2) * 4 <= SH_CUDA_KV8_WS_BYTES,
+                  "workspace: two partial items per CTA");
+    auto kernel = k_attn_kv8_tiles<DH, FP8>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TilesSmem<DH>::kBytes);
+    if (e != cudaSuccess) return e;
+    return sh::launch_pdl(kernel, dim3(sms), dim3(kTlThreads), TilesSmem<DH>::kBytes, st, mk, mv, a);
 }
 
 // K or V codes as [pages, heads * page, dh] bytes: boxes of 16 tokens of one page and head
@@ -654,6 +1182,7 @@ int sh_cuda_attention_kv8(uint64_t q, uint64_t o, const sh_cuda_kv8_t *c, uint64
     a.ld_table = ld_table, a.R = R, a.T = T, a.G = H / c->heads, a.heads = c->heads, a.pages = c->pages;
     a.page_shift = sh::kv8_shift(c->page), a.ldq = ldq, a.ldo = ldo, a.sl2 = scale * 1.4426950408889634f;
     a.vec = sh::aligned16(q) && ldq % 8 == 0 && (o & 3) == 0 && ldo % 2 == 0;
+    a.vec_o = sh::aligned16(o) && ldo % 8 == 0;
     a.counters = (uint32_t *)ws, a.part = (float *)(ws + kCounterBytes), a.err = s.dev_err;
     const int sms = s.num_sms < (int)kMaxSms ? s.num_sms : (int)kMaxSms;
     const bool fp8 = c->fmt == SH_FP8, wide = (uint64_t)max_q * a.G > 8;
@@ -670,7 +1199,12 @@ int sh_cuda_attention_kv8(uint64_t q, uint64_t o, const sh_cuda_kv8_t *c, uint64
     const bool few = (uint64_t)R * c->heads < (uint64_t)sms;
 #define SH_KV8(dh, nt, n) \
     (fp8 ? launch_rows<dh, nt, n, true>(a, mk, mv, sms, s.stream) : launch_rows<dh, nt, n, false>(a, mk, mv, sms, s.stream))
-    if (c->dh == 64) e = wide ? SH_KV8(64, 2, 4) : few ? SH_KV8(64, 1, 8) : SH_KV8(64, 1, 4);
+    // 64 rows are four tiles of the kernel above: 16 requests of 7 drafts (28 rows) 51 us there, 96 us here; 4 of 64 (256 rows)
+    // 107 us there, 68 us here.
+    if ((uint64_t)max_q * a.G > 64) {
+        if (c->dh == 64) e = fp8 ? launch_tiles<64, true>(a, mk, mv, sms, s.stream) : launch_tiles<64, false>(a, mk, mv, sms, s.stream);
+        else e = fp8 ? launch_tiles<128, true>(a, mk, mv, sms, s.stream) : launch_tiles<128, false>(a, mk, mv, sms, s.stream);
+    } else if (c->dh == 64) e = wide ? SH_KV8(64, 2, 4) : few ? SH_KV8(64, 1, 8) : SH_KV8(64, 1, 4);
     else e = wide ? SH_KV8(128, 2, 4) : few ? SH_KV8(128, 1, 8) : SH_KV8(128, 1, 4);
 #undef SH_KV8
     return sh::cuda_ok(e, "sh_cuda_attention_kv8") ? 0 : -1;
