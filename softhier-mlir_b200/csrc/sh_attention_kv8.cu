@@ -23,6 +23,7 @@ struct KvArgs {
     float sl2;            // scale * log2(e)
     uint32_t vec;         // q rows take 16-byte loads, o rows 4-byte stores
     uint32_t vec_o;       // o rows take 16-byte stores
+    uint32_t flip;        // sign bits to turn in q: the scale is negative (sl2 is its magnitude then; tiles only)
     uint32_t *counters;   // arrivals per CTA whose last item goes on in others, zero between calls
     float *part;
     int *err;
@@ -599,8 +600,8 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
 //                 this one, for one tile after the other keeps one tile's matrix products under the other's softmax.
 //   warps 4..7    turn a block's codes into fp16 operands in the swizzled layout of the matrix unit, once for both tiles
 //                 (one key row per lane: neither the reads nor the writes of a quarter-warp meet in a bank)
-//   warps 8..15   softmax, one row per thread (8..11 tile 0, 12..15 tile 1), the scores read from tensor memory twice, for
-//                 the maximum and for the weights, so that 512 threads fit the register file
+//   warps 8..15   softmax, one row per thread (8..11 tile 0, 12..15 tile 1), a row's 128 scores in registers: 184 of them
+//                 against 72 for the other warps (512 threads start with 128 each: 256 x 184 + 256 x 72 = 512 x 128)
 // The scales of 16 tokens are one multiply-add per score (x = ks s + log2 vs) and one per 16 weights. A block is 2048 cycles of
 // tensor work and as many of the special-function unit's (32768 exponentials).
 // ================================================================================================================
@@ -615,6 +616,12 @@ struct TilesSmem {
     static constexpr uint32_t kGroup = kInfo + kTlStages * 128;        // [2][8] {ks scale log2 e, log2 vs, 1 / vs}
     static constexpr uint32_t kBars = kGroup + 256, kMisc = kBars + 32 * 8, kBytes = kMisc + 256 + 1024;
 };
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 
 // A tile of a request in the run of a CTA
 struct TileCursor {
@@ -751,108 +758,114 @@ __global__ void __launch_bounds__(kTlThreads, 1)
         k0.b = (uint32_t)(in - before);
     }
 
-    if (warp == 0) {
-        // ---------------- copies: lane i has tokens 16 i .. of a block ----------------
-        TileCursor k = k0;
-        uint32_t st = 0, ph = 0, n = 0;
-        auto lookup = [&]() {
-            const uint32_t tok = k.b * kTlKeys + lane * 16;
-            return lane < 8 && (int)tok < k.lim_hi ? a.table[(size_t)k.r * a.ld_table + (tok >> a.page_shift)] : -1;
-        };
-        int id = begin < end ? lookup() : -1;
-        for (u64 u = begin; u < end; ++u, ++n) {
-            const uint32_t tok = k.b * kTlKeys + lane * 16;
-            const bool used = lane < 8 && (int)tok < k.lim_hi, ok = used && (uint32_t)id < a.pages;
-            const int row = (int)((k.kvh << a.page_shift) + (tok & page1)), page = id;
-            const size_t at = (size_t)(uint32_t)id * a.heads + k.kvh;
-            if (u + 1 < end) {
-                if (++k.b == k.blocks) tile_next(k, a);
-                id = lookup();
-            }
-            if (n >= kTlStages) mbar_wait(c_empty + st, ph ^ 1u, abort, a.err);
-            uint64_t *bar = c_full + st;
-            const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, ok));
-            if (lane == 0) mbar_arrive_expect_tx(bar, boxes * 2 * SM::kBox);
-            __syncwarp();
-            if (lane < 8) {
-                float *info = reinterpret_cast<float *>(sm + SM::kInfo + (st * 8 + lane) * 16);
-                info[2] = ok;
-                if (ok) {
-                    uint8_t *dst = sm + SM::kRing + st * 2 * SM::kCodes + lane * SM::kBox;
-                    tma_load_3d(dst, &mk, bar, 0, row, page);
-                    tma_load_3d(dst + SM::kCodes, &mv, bar, 0, row, page);
-                    cp_async4(smem_u32(info), a.ks + at);
-                    cp_async4(smem_u32(info) + 4, a.vs + at);
-                } else if (used) {
-                    atomicCAS(a.err, 0, (int)sh::kErrBadArgs);
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 0) {
+            // ---------------- copies: lane i has tokens 16 i .. of a block ----------------
+            TileCursor k = k0;
+            uint32_t st = 0, ph = 0, n = 0;
+            auto lookup = [&]() {
+                const uint32_t tok = k.b * kTlKeys + lane * 16;
+                return lane < 8 && (int)tok < k.lim_hi ? a.table[(size_t)k.r * a.ld_table + (tok >> a.page_shift)] : -1;
+            };
+            int id = begin < end ? lookup() : -1;
+            for (u64 u = begin; u < end; ++u, ++n) {
+                const uint32_t tok = k.b * kTlKeys + lane * 16;
+                const bool used = lane < 8 && (int)tok < k.lim_hi, ok = used && (uint32_t)id < a.pages;
+                const int row = (int)((k.kvh << a.page_shift) + (tok & page1)), page = id;
+                const size_t at = (size_t)(uint32_t)id * a.heads + k.kvh;
+                if (u + 1 < end) {
+                    if (++k.b == k.blocks) tile_next(k, a);
+                    id = lookup();
                 }
-                cp_async_arrive(bar);
-            }
-            if (++st == kTlStages) st = 0, ph ^= 1u;
-        }
-        // every copy has landed before the CTA may exit
-        for (uint32_t i = 0; i < min(n, kTlStages); ++i) {
-            const uint32_t last = n - 1 - i;
-            if (lane == 0) drain_wait(c_full + last % kTlStages, last / kTlStages & 1);
-        }
-    } else if (warp == 1) {
-        // ---------------- MMA issue: the whole warp walks the loop, lane 0 issues ----------------
-        const uint32_t is0 = lane == 0 ? 1u : 0u;
-        constexpr uint32_t idesc_s = umma_idesc_f16(kTlRows, kTlKeys, 0, 0), idesc_o = umma_idesc_f16(kTlRows, DH, 0, 1);
-        const uint64_t qd = sw128_desc(smem_u32(sm + SM::kQ), 16, 1024), kd = sw128_desc(smem_u32(sm + SM::kK), 16, 1024);
-        const uint64_t vd = sw128_desc(smem_u32(sm + SM::kV), SM::kChunk, 1024);
-        uint32_t kn = 0, vn = 0, pn[2] = {0, 0}, qn[2] = {0, 0};      // phases seen of each barrier
-        TileCursor k = k0;
-        for (u64 u = begin; u < end;) {
-            const uint32_t nb = (uint32_t)min((u64)(k.blocks - k.b), end - u), nt = k.nrows > kTlRows ? 2u : 1u;
-            // step j: P V of block j - 1, S of block j
-            for (uint32_t j = 0; j <= nb; ++j) {
-                if (j > 0) mbar_wait(v_full, vn++ & 1u, abort, a.err);
-                if (j < nb) mbar_wait(k_full, kn++ & 1u, abort, a.err);
-#pragma unroll 1
-                for (uint32_t t2 = 0; t2 < nt; ++t2) {
-                    if (j > 0) {
-                        mbar_wait(p_full + t2, pn[t2]++ & 1u, abort, a.err);
-                        tc_fence_after();
-#pragma unroll
-                        for (int i = 0; i < (int)kTlKeys / 16; ++i)
-                            umma_f16_ts_if(is0, tmem + kTmO + t2 * DH, tmem + kTmS + t2 * kTlKeys + i * 8,
-                                           vd + (uint64_t)(i * (2048 >> 4)), idesc_o, (j == 1 && i == 0) ? 0u : 1u);
-                        if (j == nb) umma_commit_if(is0, o_full + t2);
+                if (n >= kTlStages) mbar_wait(c_empty + st, ph ^ 1u, abort, a.err);
+                uint64_t *bar = c_full + st;
+                const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, ok));
+                if (lane == 0) mbar_arrive_expect_tx(bar, boxes * 2 * SM::kBox);
+                __syncwarp();
+                if (lane < 8) {
+                    float *info = reinterpret_cast<float *>(sm + SM::kInfo + (st * 8 + lane) * 16);
+                    info[2] = ok;
+                    if (ok) {
+                        uint8_t *dst = sm + SM::kRing + st * 2 * SM::kCodes + lane * SM::kBox;
+                        tma_load_3d(dst, &mk, bar, 0, row, page);
+                        tma_load_3d(dst + SM::kCodes, &mv, bar, 0, row, page);
+                        cp_async4(smem_u32(info), a.ks + at);
+                        cp_async4(smem_u32(info) + 4, a.vs + at);
+                    } else if (used) {
+                        atomicCAS(a.err, 0, (int)sh::kErrBadArgs);
                     }
-                    if (j < nb) {
-                        if (j == 0) mbar_wait(q_full + t2, qn[t2]++ & 1u, abort, a.err);
-                        tc_fence_after();
-#pragma unroll
-                        for (int i = 0; i < DH / 16; ++i) {
-                            const uint32_t at = ((uint32_t)(i / 4) * SM::kChunk + (i % 4) * 32) >> 4;
-                            umma_f16_ss_if(is0, tmem + kTmS + t2 * kTlKeys, qd + (t2 * SM::kTile >> 4) + at, kd + at, idesc_s,
-                                           i > 0 ? 1u : 0u);
+                    cp_async_arrive(bar);
+                }
+                if (++st == kTlStages) st = 0, ph ^= 1u;
+            }
+            // every copy has landed before the CTA may exit
+            for (uint32_t i = 0; i < min(n, kTlStages); ++i) {
+                const uint32_t last = n - 1 - i;
+                if (lane == 0) drain_wait(c_full + last % kTlStages, last / kTlStages & 1);
+            }
+        } else if (warp == 1) {
+            // ---------------- MMA issue: the whole warp walks the loop, lane 0 issues ----------------
+            const uint32_t is0 = lane == 0 ? 1u : 0u;
+            constexpr uint32_t idesc_s = umma_idesc_f16(kTlRows, kTlKeys, 0, 0), idesc_o = umma_idesc_f16(kTlRows, DH, 0, 1);
+            const uint64_t qd = sw128_desc(smem_u32(sm + SM::kQ), 16, 1024), kd = sw128_desc(smem_u32(sm + SM::kK), 16, 1024);
+            const uint64_t vd = sw128_desc(smem_u32(sm + SM::kV), SM::kChunk, 1024);
+            uint32_t kn = 0, vn = 0, pn[2] = {0, 0}, qn[2] = {0, 0};      // phases seen of each barrier
+            TileCursor k = k0;
+            for (u64 u = begin; u < end;) {
+                const uint32_t nb = (uint32_t)min((u64)(k.blocks - k.b), end - u), nt = k.nrows > kTlRows ? 2u : 1u;
+                // step j: P V of block j - 1, S of block j
+                for (uint32_t j = 0; j <= nb; ++j) {
+                    if (j > 0) mbar_wait(v_full, vn++ & 1u, abort, a.err);
+                    if (j < nb) mbar_wait(k_full, kn++ & 1u, abort, a.err);
+    #pragma unroll 1
+                    for (uint32_t t2 = 0; t2 < nt; ++t2) {
+                        if (j > 0) {
+                            mbar_wait(p_full + t2, pn[t2]++ & 1u, abort, a.err);
+                            tc_fence_after();
+    #pragma unroll
+                            for (int i = 0; i < (int)kTlKeys / 16; ++i)
+                                umma_f16_ts_if(is0, tmem + kTmO + t2 * DH, tmem + kTmS + t2 * kTlKeys + i * 8,
+                                               vd + (uint64_t)(i * (2048 >> 4)), idesc_o, (j == 1 && i == 0) ? 0u : 1u);
+                            if (j == nb) umma_commit_if(is0, o_full + t2);
                         }
-                        umma_commit_if(is0, s_full + t2);
+                        if (j < nb) {
+                            if (j == 0) mbar_wait(q_full + t2, qn[t2]++ & 1u, abort, a.err);
+                            tc_fence_after();
+    #pragma unroll
+                            for (int i = 0; i < DH / 16; ++i) {
+                                const uint32_t at = ((uint32_t)(i / 4) * SM::kChunk + (i % 4) * 32) >> 4;
+                                umma_f16_ss_if(is0, tmem + kTmS + t2 * kTlKeys, qd + (t2 * SM::kTile >> 4) + at, kd + at, idesc_s,
+                                               i > 0 ? 1u : 0u);
+                            }
+                            umma_commit_if(is0, s_full + t2);
+                        }
                     }
+                    if (j > 0) umma_commit_if(is0, v_empty);
+                    if (j < nb) umma_commit_if(is0, k_empty);
                 }
-                if (j > 0) umma_commit_if(is0, v_empty);
-                if (j < nb) umma_commit_if(is0, k_empty);
+                u += nb;
+                if (u < end) tile_next(k, a);
             }
-            u += nb;
-            if (u < end) tile_next(k, a);
+            // tensor memory may only be freed once every issued MMA has completed
+            umma_commit_if(is0, mdone);
+            if (is0) drain_wait(mdone, 0);
         }
-        // tensor memory may only be freed once every issued MMA has completed
-        umma_commit_if(is0, mdone);
-        if (is0) drain_wait(mdone, 0);
-    } else if (warp >= 4 && warp < 8) {
+    } else if (warp < 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         // ---------------- codes -> fp16: lane has key row 32 (warp - 4) + lane ----------------
         const uint32_t row = (warp - 4) * 32 + lane, grp = row >> 4;
         uint32_t st = 0, ph = 0, n = 0;
         TileCursor k = k0;
         auto convert = [&](const uint8_t *src, uint8_t *dst, bool keep) {
+            // 16 codes: piece p of the row in the ring's swizzle; 32 bytes of fp16: pieces 2 p, 2 p + 1 of a 64-column chunk
+            uint4 x[DH / 16];
+#pragma unroll
+            for (int p = 0; p < DH / 16; ++p)
+                x[p] = lds16(smem_u32(src) + row * DH + (DH == 128 ? (p ^ (row & 7)) : (p ^ (row >> 1 & 3))) * 16);
 #pragma unroll
             for (int p = 0; p < DH / 16; ++p) {
-                // 16 codes: piece p of the row in the ring's swizzle; 32 bytes of fp16: pieces 2 p, 2 p + 1 of the 64-column chunk
-                const uint32_t pos = DH == 128 ? (p ^ (row & 7)) : (p ^ (row >> 1 & 3));
-                const uint4 x = lds16(smem_u32(src) + row * DH + pos * 16);
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                const uint32_t w[4] = {x[p].x, x[p].y, x[p].z, x[p].w};
                 uint32_t h[8];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -884,7 +897,8 @@ __global__ void __launch_bounds__(kTlThreads, 1)
             if ((lane & 15) == 0) {
                 const float vs = ok ? fmaxf(info.y, 0x1p-80f) : 1.f;
                 *reinterpret_cast<float4 *>(sm + SM::kGroup + ((n & 1) * 8 + grp) * 16) =
-                    make_float4(ok ? info.x * a.sl2 : 0.f, ok ? __log2f(vs) : -INFINITY, __frcp_rn(vs), 0.f);
+                    make_float4(fmaxf(ok ? info.x * a.sl2 : 0.f, 0x1p-100f), ok ? __log2f(vs) : -INFINITY, __frcp_rn(vs), 0.f);   // > 0: a
+                    // masked score of -infinity stays that
             }
             convert(codes, sm + SM::kK, ok);
             if (lane == 0) mbar_arrive(k_full);
@@ -895,7 +909,8 @@ __global__ void __launch_bounds__(kTlThreads, 1)
             if (++st == kTlStages) st = 0, ph ^= 1u;
             if (u + 1 < end && ++k.b == k.blocks) tile_next(k, a);
         }
-    } else if (warp >= 8) {
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
         // ---------------- softmax and output ----------------
         const uint32_t t2 = (warp - 8) >> 2, quarter = warp & 3, row = quarter * 32 + lane;      // row of the tile
         const uint32_t st = t - 256;                                                              // of 256 softmax threads
@@ -929,6 +944,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                             x = make_uint4(w[0], w[1], w[2], w[3]);
                         }
                     }
+                    x.x ^= a.flip, x.y ^= a.flip, x.z ^= a.flip, x.w ^= a.flip;
                     *reinterpret_cast<uint4 *>(to + (p >> 3) * SM::kChunk + (((p & 7) ^ (row & 7)) * 16)) = x;
                 }
                 fence_proxy_async_smem();
@@ -941,33 +957,37 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                 const float4 *grp = reinterpret_cast<const float4 *>(sm + SM::kGroup + (n & 1) * 128);
                 mbar_wait(s_full + t2, sn++ & 1u, abort, a.err);      // and P V of the block before is complete
                 tc_fence_after();
-                const bool edge = key0 + (int)kTlKeys > lim_lo;
-                // exponents of 32 keys: x = s ks scale log2 e + log2 vs
-                auto exponents = [&](const uint32_t (&v)[32], float (&x)[32], int c) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float4 gr = grp[2 * c + h];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) x[16 * h + i] = fmaf(__uint_as_float(v[16 * h + i]), gr.x, gr.y);
-                    }
-                    if (edge) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (key0 + 32 * c + i >= lim) x[i] = -INFINITY;
-                    }
-                };
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t v[32];
-                    float x[32];
-                    tmem_ld_32x32b_x32(s_addr + 32 * c, v);
+                float sc[kTlKeys];
+                {
+                    uint32_t v0[32], v1[32], v2[32], v3[32];   // four loads in flight, one wait
+                    tmem_ld_32x32b_x32(s_addr, v0);
+                    tmem_ld_32x32b_x32(s_addr + 32, v1);
+                    tmem_ld_32x32b_x32(s_addr + 64, v2);
+                    tmem_ld_32x32b_x32(s_addr + 96, v3);
                     tmem_ld_wait();
-                    exponents(v, x, c);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], x[i]);
+                    for (int i = 0; i < 32; ++i) {
+                        sc[i] = __uint_as_float(v0[i]);
+                        sc[32 + i] = __uint_as_float(v1[i]);
+                        sc[64 + i] = __uint_as_float(v2[i]);
+                        sc[96 + i] = __uint_as_float(v3[i]);
+                    }
                 }
-                const float mb = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                if (key0 + (int)kTlKeys > lim_lo) {
+#pragma unroll
+                    for (int i = 0; i < (int)kTlKeys; ++i)
+                        if (key0 + i >= lim) sc[i] = -INFINITY;
+                }
+                // 16 keys share their scales (>= 0): the largest exponent comes from the largest score
+                float mb = -INFINITY;
+#pragma unroll
+                for (int h = 0; h < 8; ++h) {
+                    const float4 gr = grp[h];
+                    const float *x = sc + 16 * h;
+                    const float a0 = max3(x[0], x[1], x[2]), a1 = max3(x[3], x[4], x[5]), a2 = max3(x[6], x[7], x[8]);
+                    const float a3 = max3(x[9], x[10], x[11]), a4 = max3(x[12], x[13], x[14]);
+                    mb = fmaxf(mb, fmaf(max3(max3(a0, a1, a2), fmaxf(a3, a4), x[15]), gr.x, gr.y));
+                }
                 // the maximum only moves when a weight would pass 2^8 (exact room in fp16); O is rescaled then
                 float alpha = 1.f;
                 const bool raise = mb > m + 8.f;
@@ -990,23 +1010,22 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                 const float ms = m == -INFINITY ? 0.f : m;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    uint32_t v[32], packed[16];
-                    float x[32];
-                    tmem_ld_32x32b_x32(s_addr + 32 * c, v);
-                    tmem_ld_wait();
-                    exponents(v, x, c);
+                    uint32_t packed[16];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
+                        const float4 gr = grp[2 * c + h];
+                        const float y = gr.y - ms;
                         float s4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            const float p0 = fast_exp2(x[16 * h + 2 * i] - ms), p1 = fast_exp2(x[16 * h + 2 * i + 1] - ms);
+                            const float p0 = fast_exp2(fmaf(sc[32 * c + 16 * h + 2 * i], gr.x, y));
+                            const float p1 = fast_exp2(fmaf(sc[32 * c + 16 * h + 2 * i + 1], gr.x, y));
                             s4[(2 * i) & 3] += p0, s4[(2 * i + 1) & 3] += p1;
                             packed[8 * h + i] = pack_h2(p0, p1);
                         }
-                        l = fmaf((s4[0] + s4[1]) + (s4[2] + s4[3]), grp[2 * c + h].z, l);
+                        l = fmaf((s4[0] + s4[1]) + (s4[2] + s4[3]), gr.z, l);
                     }
-                    tmem_st_32x32b_x16(s_addr + 16 * c, packed);      // over scores that have been read
+                    tmem_st_32x32b_x16(s_addr + 16 * c, packed);      // over scores that are in registers
                 }
                 tmem_st_wait();
                 tc_fence_before();
@@ -1202,6 +1221,8 @@ int sh_cuda_attention_kv8(uint64_t q, uint64_t o, const sh_cuda_kv8_t *c, uint64
     // 64 rows are four tiles of the kernel above: 16 requests of 7 drafts (28 rows) 51 us there, 96 us here; 4 of 64 (256 rows)
     // 107 us there, 68 us here.
     if ((uint64_t)max_q * a.G > 64) {
+        a.flip = scale < 0.f ? 0x80008000u : 0u;
+        a.sl2 = fabsf(a.sl2);
         if (c->dh == 64) e = fp8 ? launch_tiles<64, true>(a, mk, mv, sms, s.stream) : launch_tiles<64, false>(a, mk, mv, sms, s.stream);
         else e = fp8 ? launch_tiles<128, true>(a, mk, mv, sms, s.stream) : launch_tiles<128, false>(a, mk, mv, sms, s.stream);
     } else if (c->dh == 64) e = wide ? SH_KV8(64, 2, 4) : few ? SH_KV8(64, 1, 8) : SH_KV8(64, 1, 4);
