@@ -593,28 +593,33 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
 
 // ================================================================================================================
 // Many rows per request (prompt chunks): tcgen05. A CTA per SM walks its run of units (request, kv head, 256 rows, block of
-// 128 tokens; the blocks behind a tile's last row are left out). 512 threads:
+// 128 tokens; the blocks behind a tile's last row are left out). 768 threads:
 //   warp 0        copies: the pages' K and V boxes (8 bits) and scales into a ring of two blocks, as above
 //   warp 1        tcgen05.mma: per block and 128-row tile t  S_t = Q_t K^T (N = 128 tokens), then, when the softmax has
 //                 written P_t over S_t, O_t += P_t V with P_t read from tensor memory. The order P V of the block before, S of
 //                 this one, for one tile after the other keeps one tile's matrix products under the other's softmax.
 //   warps 4..7    turn a block's codes into fp16 operands in the swizzled layout of the matrix unit, once for both tiles
-//                 (one key row per lane: neither the reads nor the writes of a quarter-warp meet in a bank)
-//   warps 8..15   softmax, one row per thread (8..11 tile 0, 12..15 tile 1), a row's 128 scores in registers: 184 of them
-//                 against 72 for the other warps (512 threads start with 128 each: 256 x 184 + 256 x 72 = 512 x 128)
-// The scales of 16 tokens are one multiply-add per score (x = ks s + log2 vs) and one per 16 weights. A block is 2048 cycles of
-// tensor work and as many of the special-function unit's (32768 exponentials).
+//                 (one key row per lane: neither the reads nor the writes of a quarter-warp meet in a bank); K a block ahead
+//   warps 8..23   softmax: eight warps per tile, two threads per row, each with 64 of its scores in registers. A tile's
+//                 products wait for its weights and its scores for its products, so the softmax's latency counts: with one
+//                 thread per row a block took 5000 cycles.
+// The scales of 16 tokens are one multiply-add per 16 scores for the maximum, one per score (x = ks s + log2 vs) and one per
+// 16 weights. A block is 2048 cycles of tensor work at its peak rate and as many of the special-function unit's (32768
+// exponentials); 32 matrix instructions of about 100 cycles each are what it cannot go below in this shape.
 // ================================================================================================================
-constexpr uint32_t kTlRows = 128, kTlKeys = 128, kTlItem = 256, kTlThreads = 512, kTlStages = 2;
+constexpr uint32_t kTlRows = 128, kTlKeys = 128, kTlItem = 256, kTlThreads = 768, kTlStages = 2;
+constexpr uint32_t kTlRegs = 96, kTlRegsOther = 48;      // 512 x 96 + 256 x 48 = 768 x 80, what the block starts with
 
 template <int DH>
 struct TilesSmem {
     static constexpr uint32_t kChunk = 128 * 128;                      // 128 rows x 64 fp16 columns
     static constexpr uint32_t kTile = DH / 64 * kChunk, kBox = 16 * DH, kCodes = kTlKeys * DH;
-    static constexpr uint32_t kQ = 0, kK = kQ + 2 * kTile, kV = kK + kTile, kRing = kV + kTile;
+    static constexpr uint32_t kQ = 0, kK = kQ + 2 * kTile, kV = kK + 2 * kTile, kRing = kV + kTile;   // K twice
     static constexpr uint32_t kInfo = kRing + kTlStages * 2 * kCodes;  // [stages][8] {ks, vs, usable}
-    static constexpr uint32_t kGroup = kInfo + kTlStages * 128;        // [2][8] {ks scale log2 e, log2 vs, 1 / vs}
-    static constexpr uint32_t kBars = kGroup + 256, kMisc = kBars + 32 * 8, kBytes = kMisc + 256 + 1024;
+    static constexpr uint32_t kGroup = kInfo + kTlStages * 128;        // [4][8] {ks scale log2 e, log2 vs, 1 / vs}
+    static constexpr uint32_t kRowMax = kGroup + 512;                  // [2 tiles][2][128] bf16
+    static constexpr uint32_t kBars = kRowMax + 1024, kMisc = kBars + 24 * 8, kBytes = kMisc + 320;
+    static_assert(kBytes <= 227 * 1024, "shared memory");
 };
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -660,16 +665,20 @@ __global__ void __launch_bounds__(kTlThreads, 1)
     using SM = TilesSmem<DH>;
     typedef unsigned long long u64;
     constexpr uint32_t kTmS = 0, kTmO = 2 * kTlKeys;                   // tensor memory: S_t / P_t, O_t
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t *sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    extern __shared__ __align__(1024) uint8_t tiles_smem[];      // swizzled tiles from its start: no room to align by hand
+    uint8_t *sm = tiles_smem;
+    if (smem_u32(sm) & 1023u) {
+        if (threadIdx.x == 0) atomicCAS(a.err, 0, (int)sh::kErrBadArgs);
+        return;
+    }
     uint64_t *bars = reinterpret_cast<uint64_t *>(sm + SM::kBars);
     uint64_t *c_full = bars, *c_empty = bars + 2;                      // ring of codes
-    uint64_t *k_full = bars + 4, *k_empty = bars + 5, *v_full = bars + 6, *v_empty = bars + 7;
+    uint64_t *k_full = bars + 4, *k_empty = bars + 18, *v_full = bars + 6, *v_empty = bars + 7;   // K: two each
     uint64_t *q_full = bars + 8, *s_full = bars + 10, *p_full = bars + 12, *o_full = bars + 14, *mdone = bars + 16;
     struct Misc {
         u64 part[kTlThreads / 32];
-        u64 off;
-        uint32_t r, flag, tmem;
+        TileCursor first;
+        uint32_t flag, tmem;
         int abort;
     };
     Misc &mi = *reinterpret_cast<Misc *>(sm + SM::kMisc);
@@ -679,9 +688,10 @@ __global__ void __launch_bounds__(kTlThreads, 1)
     if (t == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(c_full + i, 1 + 8), mbar_init(c_empty + i, 4);
-            mbar_init(q_full + i, 4), mbar_init(s_full + i, 1), mbar_init(p_full + i, 4), mbar_init(o_full + i, 1);
+            mbar_init(k_full + i, 4), mbar_init(k_empty + i, 1);
+            mbar_init(q_full + i, 8), mbar_init(s_full + i, 1), mbar_init(p_full + i, 8), mbar_init(o_full + i, 1);
         }
-        mbar_init(k_full, 4), mbar_init(k_empty, 1), mbar_init(v_full, 4), mbar_init(v_empty, 1), mbar_init(mdone, 1);
+        mbar_init(v_full, 4), mbar_init(v_empty, 1), mbar_init(mdone, 1);
         mi.abort = 0;
         prefetch_tmap(&mk), prefetch_tmap(&mv);
         fence_mbar_init();
@@ -698,25 +708,22 @@ __global__ void __launch_bounds__(kTlThreads, 1)
     pdl_wait();
 
     // ---- this CTA's run of units ------------------------------------------------------------------------------------
-    auto request_units = [&](uint32_t r, u64 stop, u64 &off) -> u64 {      // units of one head; stops in the tile that holds `stop`
-        TileCursor k;
-        k.r = r;
-        tile_request(k, a);
+    auto head_units = [&](TileCursor &k) {      // units of one head of a request
         u64 n = 0;
         for (k.tile = 0; k.tile < k.tiles; ++k.tile) {
             tile_sizes(k, a);
-            if (n + k.blocks > stop) {
-                off = n;
-                return k.tile;
-            }
             n += k.blocks;
         }
         return n;
     };
     const uint32_t per_t = (a.R + kTlThreads - 1) / kTlThreads, r0 = min(t * per_t, a.R), r1 = min(r0 + per_t, a.R);
-    u64 sum = 0, none;
+    TileCursor k0 = {};
+    u64 sum = 0, one = 0;
     for (uint32_t r = r0; r < r1; ++r) {
-        sum += a.heads * request_units(r, ~0ull, none);
+        k0.r = r;
+        tile_request(k0, a);
+        one = head_units(k0);
+        sum += a.heads * one;
         if (blockIdx.x == 0 && a.lens[r] > (int)(a.ld_table << a.page_shift)) atomicCAS(a.err, 0, (int)sh::kErrBadArgs);
     }
     u64 incl = sum;
@@ -736,30 +743,25 @@ __global__ void __launch_bounds__(kTlThreads, 1)
     if (begin < end && begin >= incl - sum && begin < incl) {
         u64 off = begin - (incl - sum);
         for (uint32_t r = r0; r < r1; ++r) {
-            const u64 n = a.heads * request_units(r, ~0ull, none);
-            if (off < n) {
-                mi.r = r, mi.off = off;
-                break;
+            if (r1 - r0 > 1) {
+                k0.r = r;
+                tile_request(k0, a);
+                one = head_units(k0);
             }
-            off -= n;
+            if (off < a.heads * one) break;
+            off -= a.heads * one;
         }
+        k0.kvh = (uint32_t)(off / one);
+        off -= k0.kvh * one;
+        for (k0.tile = 0; tile_sizes(k0, a), off >= k0.blocks; ++k0.tile) off -= k0.blocks;
+        k0.b = (uint32_t)off;
+        mi.first = k0;
     }
     __syncthreads();
-    TileCursor k0 = {};
-    if (begin < end) {
-        k0.r = mi.r;
-        const u64 one = request_units(k0.r, ~0ull, none);
-        k0.kvh = (uint32_t)(mi.off / one);
-        u64 before = 0;
-        const u64 in = mi.off - k0.kvh * one;
-        k0.tile = (uint32_t)request_units(k0.r, in, before);
-        tile_request(k0, a);
-        tile_sizes(k0, a);
-        k0.b = (uint32_t)(in - before);
-    }
+    k0 = mi.first;
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTlRegsOther));
         if (warp == 0) {
             // ---------------- copies: lane i has tokens 16 i .. of a block ----------------
             TileCursor k = k0;
@@ -817,7 +819,8 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                 // step j: P V of block j - 1, S of block j
                 for (uint32_t j = 0; j <= nb; ++j) {
                     if (j > 0) mbar_wait(v_full, vn++ & 1u, abort, a.err);
-                    if (j < nb) mbar_wait(k_full, kn++ & 1u, abort, a.err);
+                    const uint32_t ks = kn & 1u;      // K's buffer
+                    const uint64_t kdj = kd + (ks * SM::kTile >> 4);
     #pragma unroll 1
                     for (uint32_t t2 = 0; t2 < nt; ++t2) {
                         if (j > 0) {
@@ -828,21 +831,22 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                                 umma_f16_ts_if(is0, tmem + kTmO + t2 * DH, tmem + kTmS + t2 * kTlKeys + i * 8,
                                                vd + (uint64_t)(i * (2048 >> 4)), idesc_o, (j == 1 && i == 0) ? 0u : 1u);
                             if (j == nb) umma_commit_if(is0, o_full + t2);
+                            if (t2 + 1 == nt) umma_commit_if(is0, v_empty);
                         }
                         if (j < nb) {
+                            if (t2 == 0) mbar_wait(k_full + ks, kn >> 1 & 1u, abort, a.err);
                             if (j == 0) mbar_wait(q_full + t2, qn[t2]++ & 1u, abort, a.err);
                             tc_fence_after();
     #pragma unroll
                             for (int i = 0; i < DH / 16; ++i) {
                                 const uint32_t at = ((uint32_t)(i / 4) * SM::kChunk + (i % 4) * 32) >> 4;
-                                umma_f16_ss_if(is0, tmem + kTmS + t2 * kTlKeys, qd + (t2 * SM::kTile >> 4) + at, kd + at, idesc_s,
+                                umma_f16_ss_if(is0, tmem + kTmS + t2 * kTlKeys, qd + (t2 * SM::kTile >> 4) + at, kdj + at, idesc_s,
                                                i > 0 ? 1u : 0u);
                             }
                             umma_commit_if(is0, s_full + t2);
                         }
                     }
-                    if (j > 0) umma_commit_if(is0, v_empty);
-                    if (j < nb) umma_commit_if(is0, k_empty);
+                    if (j < nb) umma_commit_if(is0, k_empty + ks), ++kn;
                 }
                 u += nb;
                 if (u < end) tile_next(k, a);
@@ -852,73 +856,88 @@ __global__ void __launch_bounds__(kTlThreads, 1)
             if (is0) drain_wait(mdone, 0);
         }
     } else if (warp < 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTlRegsOther));
         // ---------------- codes -> fp16: lane has key row 32 (warp - 4) + lane ----------------
         const uint32_t row = (warp - 4) * 32 + lane, grp = row >> 4;
-        uint32_t st = 0, ph = 0, n = 0;
+        uint32_t n = 0;
         TileCursor k = k0;
         auto convert = [&](const uint8_t *src, uint8_t *dst, bool keep) {
             // 16 codes: piece p of the row in the ring's swizzle; 32 bytes of fp16: pieces 2 p, 2 p + 1 of a 64-column chunk
-            uint4 x[DH / 16];
 #pragma unroll
-            for (int p = 0; p < DH / 16; ++p)
-                x[p] = lds16(smem_u32(src) + row * DH + (DH == 128 ? (p ^ (row & 7)) : (p ^ (row >> 1 & 3))) * 16);
-#pragma unroll
-            for (int p = 0; p < DH / 16; ++p) {
-                const uint32_t w[4] = {x[p].x, x[p].y, x[p].z, x[p].w};
-                uint32_t h[8];
+            for (int q = 0; q < DH / 64; ++q) {
+                uint4 x[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    if (FP8) {
-                        h[2 * i] = e4m3x2_to_h2(w[i] & 0xFFFFu), h[2 * i + 1] = e4m3x2_to_h2(w[i] >> 16);
-                    } else {
-                        const uint32_t y = w[i] ^ 0x80808080u;
-                        h[2 * i] = hsub2(__byte_perm(y, 0x64646464u, 0x4140), kMagicVal);
-                        h[2 * i + 1] = hsub2(__byte_perm(y, 0x64646464u, 0x4342), kMagicVal);
-                    }
+                    const uint32_t p = q * 4 + i;
+                    x[i] = lds16(smem_u32(src) + row * DH + (DH == 128 ? (p ^ (row & 7)) : (p ^ (row >> 1 & 3))) * 16);
                 }
-                if (!keep)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) h[i] = 0;
-                uint8_t *to = dst + (p >> 2) * SM::kChunk + row * 128;
-                const uint32_t piece = (p & 3) * 2;
-                *reinterpret_cast<uint4 *>(to + ((piece ^ (row & 7)) * 16)) = make_uint4(h[0], h[1], h[2], h[3]);
-                *reinterpret_cast<uint4 *>(to + (((piece + 1) ^ (row & 7)) * 16)) = make_uint4(h[4], h[5], h[6], h[7]);
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+                    uint32_t h[8];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (FP8) {
+                            h[2 * i] = e4m3x2_to_h2(w[i] & 0xFFFFu), h[2 * i + 1] = e4m3x2_to_h2(w[i] >> 16);
+                        } else {
+                            const uint32_t y = w[i] ^ 0x80808080u;
+                            h[2 * i] = hsub2(__byte_perm(y, 0x64646464u, 0x4140), kMagicVal);
+                            h[2 * i + 1] = hsub2(__byte_perm(y, 0x64646464u, 0x4342), kMagicVal);
+                        }
+                    }
+                    if (!keep)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) h[i] = 0;
+                    uint8_t *to = dst + q * SM::kChunk + row * 128;
+                    *reinterpret_cast<uint4 *>(to + (((2 * j) ^ (row & 7)) * 16)) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4 *>(to + (((2 * j + 1) ^ (row & 7)) * 16)) = make_uint4(h[4], h[5], h[6], h[7]);
+                }
             }
             fence_proxy_async_smem();
             __syncwarp();
         };
-        for (u64 u = begin; u < end; ++u, ++n) {
-            mbar_wait(c_full + st, ph, abort, a.err);
+        // K of block n + 1 goes before V of block n: K has two buffers, so it is ready while the matrix unit is still at block n
+        auto keys = [&](uint32_t i) {
+            const uint32_t st = i & 1;
+            mbar_wait(c_full + st, i >> 1 & 1, abort, a.err);
             const float4 info = *reinterpret_cast<const float4 *>(sm + SM::kInfo + (st * 8 + grp) * 16);
             const bool ok = info.z != 0.f;
-            const uint8_t *codes = sm + SM::kRing + st * 2 * SM::kCodes;
-            if (n > 0) mbar_wait(k_empty, (n - 1) & 1u, abort, a.err);
+            if (i >= 2) mbar_wait(k_empty + st, (i >> 1 & 1) ^ 1u, abort, a.err);
             if ((lane & 15) == 0) {
                 const float vs = ok ? fmaxf(info.y, 0x1p-80f) : 1.f;
-                *reinterpret_cast<float4 *>(sm + SM::kGroup + ((n & 1) * 8 + grp) * 16) =
-                    make_float4(fmaxf(ok ? info.x * a.sl2 : 0.f, 0x1p-100f), ok ? __log2f(vs) : -INFINITY, __frcp_rn(vs), 0.f);   // > 0: a
-                    // masked score of -infinity stays that
+                // the first factor > 0: a masked score of -infinity stays that
+                *reinterpret_cast<float4 *>(sm + SM::kGroup + ((i & 3) * 8 + grp) * 16) =
+                    make_float4(fmaxf(ok ? info.x * a.sl2 : 0.f, 0x1p-100f), ok ? __log2f(vs) : -INFINITY, __frcp_rn(vs), 0.f);
             }
-            convert(codes, sm + SM::kK, ok);
-            if (lane == 0) mbar_arrive(k_full);
+            convert(sm + SM::kRing + st * 2 * SM::kCodes, sm + SM::kK + st * SM::kTile, ok);
+            if (lane == 0) mbar_arrive(k_full + st);
+        };
+        if (begin < end) keys(0);
+        for (u64 u = begin; u < end; ++u, ++n) {
+            const uint32_t st = n & 1;
+            if (u + 1 < end) keys(n + 1);
+            const bool ok = reinterpret_cast<const float4 *>(sm + SM::kInfo + (st * 8 + grp) * 16)->z != 0.f;
             if (n > 0) mbar_wait(v_empty, (n - 1) & 1u, abort, a.err);
             // rows that are no keys can hold anything; their weights are 0
-            convert(codes + SM::kCodes, sm + SM::kV, ok && (int)(k.b * kTlKeys + row) < k.lim_hi);
+            convert(sm + SM::kRing + (st * 2 + 1) * SM::kCodes, sm + SM::kV, ok && (int)(k.b * kTlKeys + row) < k.lim_hi);
             if (lane == 0) mbar_arrive(v_full), mbar_arrive(c_empty + st);
-            if (++st == kTlStages) st = 0, ph ^= 1u;
             if (u + 1 < end && ++k.b == k.blocks) tile_next(k, a);
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTlRegs));
         // ---------------- softmax and output ----------------
-        const uint32_t t2 = (warp - 8) >> 2, quarter = warp & 3, row = quarter * 32 + lane;      // row of the tile
-        const uint32_t st = t - 256;                                                              // of 256 softmax threads
+        const uint32_t t2 = (warp - 8) >> 3, half = (warp - 8) >> 2 & 1, quarter = warp & 3, row = quarter * 32 + lane;
+        const uint32_t st = t - 256;                                                              // of 512 softmax threads
+        constexpr uint32_t kHalfKeys = kTlKeys / 2, kHalfCols = DH / 2;
         const uint32_t lane_base = tmem + (quarter * 32u << 16);
-        const uint32_t s_addr = lane_base + kTmS + t2 * kTlKeys, o_addr = lane_base + kTmO + t2 * DH;
+        const uint32_t s_addr = lane_base + kTmS + t2 * kTlKeys, o_addr = lane_base + kTmO + t2 * DH + half * kHalfCols;
+        // [2][128] of the tile: the halves' maxima, as bf16 towards +infinity, so that both go on with the same value
+        uint16_t *row_max = reinterpret_cast<uint16_t *>(sm + SM::kRowMax) + t2 * 256 + row;
+        float *row_sum = reinterpret_cast<float *>(sm + SM::kQ + t2 * SM::kTile) + row;           // over Q at an item's end
         uint32_t n = 0, sn = 0, on = 0;      // blocks of the run, blocks of this tile, items of this tile
         TileCursor k = k0;
-        auto group_sync = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+        auto all_sync = [&]() { asm volatile("bar.sync 1, 512;" ::: "memory"); };
+        auto tile_sync = [&]() { asm volatile("bar.sync %0, 256;" ::"r"(2 + t2) : "memory"); };
         for (u64 u = begin; u < end;) {
             const uint32_t b0 = k.b, nb = (uint32_t)min((u64)(k.blocks - k.b), end - u), rr = t2 * kTlRows + row;
             const bool live = k.nrows > t2 * kTlRows, mine = rr < k.nrows;      // the tile's, this row's
@@ -928,24 +947,33 @@ __global__ void __launch_bounds__(kTlThreads, 1)
             const int lim_lo = min(max(k.v.base + (int)((k.row0 + t2 * kTlRows) / a.G) + 1, 0), ctx);
             float m = -INFINITY, l = 0.f;
             if (live) {
-                // Q row -> swizzled operand (the tile's score products of the item before have completed)
-                const __half *qp = a.q + (size_t)(k.v.qs + qi) * a.ldq + ((size_t)k.kvh * a.G + gi) * DH;
-                uint8_t *to = sm + SM::kQ + t2 * SM::kTile + row * 128;
-#pragma unroll 4
-                for (int p = 0; p < DH / 8; ++p) {
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (mine) {
-                        if (a.vec) {
-                            x = *reinterpret_cast<const uint4 *>(qp + p * 8);
-                        } else {
-                            uint32_t w[4] = {0, 0, 0, 0};
+                // Q rows -> swizzled operand, whole rows by neighbouring lanes (the tile's score products of the item before
+                // have completed). This warp has 16 of its quarter's rows.
+                const size_t own = mine ? (size_t)(k.v.qs + qi) * a.ldq + ((size_t)k.kvh * a.G + gi) * DH : ~(size_t)0;
+                constexpr int kPieces = DH / 8, kRowsPer = 32 / kPieces;
+                const uint32_t piece = lane % kPieces;
+                uint4 x[16 / kRowsPer];      // all loads before the first store
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) w[e >> 1] |= (uint32_t)__half_as_ushort(qp[p * 8 + e]) << (16 * (e & 1));
-                            x = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
+                for (int i = 0; i < 16 / kRowsPer; ++i) {
+                    const size_t at = __shfl_sync(0xffffffffu, own, half * 16 + i * kRowsPer + lane / kPieces);
+                    x[i] = make_uint4(0, 0, 0, 0);
+                    if (at == ~(size_t)0) continue;
+                    const __half *qp = a.q + at + piece * 8;
+                    if (a.vec) {
+                        x[i] = *reinterpret_cast<const uint4 *>(qp);
+                    } else {
+                        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) w[e >> 1] |= (uint32_t)__half_as_ushort(qp[e]) << (16 * (e & 1));
+                        x[i] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
-                    x.x ^= a.flip, x.y ^= a.flip, x.z ^= a.flip, x.w ^= a.flip;
-                    *reinterpret_cast<uint4 *>(to + (p >> 3) * SM::kChunk + (((p & 7) ^ (row & 7)) * 16)) = x;
+                }
+#pragma unroll
+                for (int i = 0; i < 16 / kRowsPer; ++i) {
+                    const uint32_t r = quarter * 32 + half * 16 + i * kRowsPer + lane / kPieces;
+                    *reinterpret_cast<uint4 *>(sm + SM::kQ + t2 * SM::kTile + (piece >> 3) * SM::kChunk + r * 128 +
+                                               (((piece & 7) ^ (r & 7)) * 16)) =
+                        make_uint4(x[i].x ^ a.flip, x[i].y ^ a.flip, x[i].z ^ a.flip, x[i].w ^ a.flip);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -953,41 +981,38 @@ __global__ void __launch_bounds__(kTlThreads, 1)
             }
             for (uint32_t j = 0; j < nb; ++j, ++n) {
                 if (!live) continue;
-                const int key0 = (int)((b0 + j) * kTlKeys);
-                const float4 *grp = reinterpret_cast<const float4 *>(sm + SM::kGroup + (n & 1) * 128);
+                const int key0 = (int)((b0 + j) * kTlKeys + half * kHalfKeys);
+                const float4 *grp = reinterpret_cast<const float4 *>(sm + SM::kGroup + (n & 3) * 128 + half * 64);
                 mbar_wait(s_full + t2, sn++ & 1u, abort, a.err);      // and P V of the block before is complete
                 tc_fence_after();
-                float sc[kTlKeys];
+                float sc[kHalfKeys];
                 {
-                    uint32_t v0[32], v1[32], v2[32], v3[32];   // four loads in flight, one wait
-                    tmem_ld_32x32b_x32(s_addr, v0);
-                    tmem_ld_32x32b_x32(s_addr + 32, v1);
-                    tmem_ld_32x32b_x32(s_addr + 64, v2);
-                    tmem_ld_32x32b_x32(s_addr + 96, v3);
+                    uint32_t v0[32], v1[32];   // two loads in flight, one wait
+                    tmem_ld_32x32b_x32(s_addr + half * kHalfKeys, v0);
+                    tmem_ld_32x32b_x32(s_addr + half * kHalfKeys + 32, v1);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        sc[i] = __uint_as_float(v0[i]);
-                        sc[32 + i] = __uint_as_float(v1[i]);
-                        sc[64 + i] = __uint_as_float(v2[i]);
-                        sc[96 + i] = __uint_as_float(v3[i]);
-                    }
+                    for (int i = 0; i < 32; ++i) sc[i] = __uint_as_float(v0[i]), sc[32 + i] = __uint_as_float(v1[i]);
                 }
-                if (key0 + (int)kTlKeys > lim_lo) {
+                if (key0 + (int)kHalfKeys > lim_lo) {
 #pragma unroll
-                    for (int i = 0; i < (int)kTlKeys; ++i)
+                    for (int i = 0; i < (int)kHalfKeys; ++i)
                         if (key0 + i >= lim) sc[i] = -INFINITY;
                 }
                 // 16 keys share their scales (>= 0): the largest exponent comes from the largest score
                 float mb = -INFINITY;
 #pragma unroll
-                for (int h = 0; h < 8; ++h) {
+                for (int h = 0; h < 4; ++h) {
                     const float4 gr = grp[h];
                     const float *x = sc + 16 * h;
                     const float a0 = max3(x[0], x[1], x[2]), a1 = max3(x[3], x[4], x[5]), a2 = max3(x[6], x[7], x[8]);
                     const float a3 = max3(x[9], x[10], x[11]), a4 = max3(x[12], x[13], x[14]);
                     mb = fmaxf(mb, fmaf(max3(max3(a0, a1, a2), fmaxf(a3, a4), x[15]), gr.x, gr.y));
                 }
+                const uint32_t up = (__float_as_uint(mb) + (mb > 0.f ? 0xFFFFu : 0u)) >> 16;
+                row_max[half * 128] = (uint16_t)up;
+                tile_sync();      // both halves' maxima are there, and both hold their scores: P may go over S
+                mb = fmaxf(__uint_as_float(up << 16), __uint_as_float((uint32_t)row_max[(half ^ 1) * 128] << 16));
                 // the maximum only moves when a weight would pass 2^8 (exact room in fp16); O is rescaled then
                 float alpha = 1.f;
                 const bool raise = mb > m + 8.f;
@@ -998,18 +1023,18 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                 }
                 if (j > 0 && __any_sync(0xffffffffu, raise)) {
 #pragma unroll 1
-                    for (int c = 0; c < DH / 32; ++c) {
-                        uint32_t v[32];
-                        tmem_ld_32x32b_x32(o_addr + c * 32, v);
+                    for (int c = 0; c < (int)kHalfCols / 16; ++c) {
+                        uint32_t v[16];
+                        tmem_ld_32x32b_x16(o_addr + c * 16, v);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
-                        tmem_st_32x32b_x32(o_addr + c * 32, v);
+                        for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+                        tmem_st_32x32b_x16(o_addr + c * 16, v);
                     }
                 }
                 const float ms = m == -INFINITY ? 0.f : m;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < 2; ++c) {
                     uint32_t packed[16];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
@@ -1025,89 +1050,112 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                         }
                         l = fmaf((s4[0] + s4[1]) + (s4[2] + s4[3]), gr.z, l);
                     }
-                    tmem_st_32x32b_x16(s_addr + 16 * c, packed);      // over scores that are in registers
+                    tmem_st_32x32b_x16(s_addr + half * (kHalfKeys / 2) + 16 * c, packed);
                 }
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full + t2);
+                // the other half has read row_max before it arrives at the next block's tile_sync, and that one writes after
+                // s_full, which follows both halves' arrivals here
             }
             // ---- the item's end: O / l, or partial sums of an item that other CTAs share ----
             if (live) {
                 mbar_wait(o_full + t2, on++ & 1u, abort, a.err);
                 tc_fence_after();
+                row_sum[half * 128] = l;
+                tile_sync();
+                l = row_sum[0] + row_sum[128];
+                tile_sync();      // read before the next item's Q goes there
             }
             const bool whole = b0 == 0 && nb == k.blocks;
             const uint32_t slot = 2 * blockIdx.x + (b0 == 0 ? 1 : 0);
             constexpr size_t kSlot = (size_t)kTlItem * (DH + 2);
             float *po = a.part + slot * kSlot, *pm = po + kTlItem * DH, *pl = pm + kTlItem;      // [DH][256], [256], [256]
-            __half *op = a.o + (size_t)(k.v.qs + qi) * a.ldo + ((size_t)k.kvh * a.G + gi) * DH;
-            auto write_out = [&](const float (&y)[32], int c, float inv) {
+            __half *op = a.o + (size_t)(k.v.qs + qi) * a.ldo + ((size_t)k.kvh * a.G + gi) * DH + half * kHalfCols;
+            auto write_out = [&](const float (&y)[16], int c, float inv) {
                 if (a.vec_o) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        *reinterpret_cast<uint4 *>(op + c * 32 + q * 8) =
+                    for (int q = 0; q < 2; ++q)
+                        *reinterpret_cast<uint4 *>(op + c * 16 + q * 8) =
                             make_uint4(pack_h2(y[8 * q] * inv, y[8 * q + 1] * inv), pack_h2(y[8 * q + 2] * inv, y[8 * q + 3] * inv),
                                        pack_h2(y[8 * q + 4] * inv, y[8 * q + 5] * inv),
                                        pack_h2(y[8 * q + 6] * inv, y[8 * q + 7] * inv));
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) op[c * 32 + i] = __float2half_rn(y[i] * inv);
+                    for (int i = 0; i < 16; ++i) op[c * 16 + i] = __float2half_rn(y[i] * inv);
                 }
             };
             if (live) {
                 const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll 1
-                for (int c = 0; c < DH / 32; ++c) {
-                    uint32_t v[32];
-                    float y[32];
-                    tmem_ld_32x32b_x32(o_addr + c * 32, v);
+#pragma unroll 2
+                for (int c = 0; c < (int)kHalfCols / 16; ++c) {
+                    uint32_t v[16];
+                    float y[16];
+                    tmem_ld_32x32b_x16(o_addr + c * 16, v);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(v[i]);
+                    for (int i = 0; i < 16; ++i) y[i] = __uint_as_float(v[i]);
                     if (mine) {
                         if (whole) {
                             write_out(y, c, inv);
                         } else {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) po[(size_t)(c * 32 + i) * kTlItem + rr] = y[i];
+                            for (int i = 0; i < 16; ++i) po[(size_t)(half * kHalfCols + c * 16 + i) * kTlItem + rr] = y[i];
                         }
                     }
                 }
                 tc_fence_before();
-                if (mine && !whole) pm[rr] = m, pl[rr] = l;
+                if (mine && !whole && half == 0) pm[rr] = m, pl[rr] = l;
             }
             if (!whole) {
                 const u64 i0 = u - b0;      // the item's first unit: its CTA counts the arrivals
                 const uint32_t c0 = (uint32_t)(i0 / per), c1 = (uint32_t)((i0 + k.blocks - 1) / per);
-                group_sync();
+                all_sync();
                 if (st == 0) {
                     const uint32_t before = atom_add_acq_rel_gpu(a.counters + c0, 1u);
                     mi.flag = before == c1 - c0;
                     if (mi.flag) a.counters[c0] = 0;      // for the next call
                 }
-                group_sync();
+                all_sync();
                 if (mi.flag && mine) {
                     const uint32_t parts = c1 - c0 + 1;
                     auto part = [&](uint32_t i) { return a.part + (size_t)(2 * (c0 + i) + (i == 0)) * kSlot; };
                     float mt = -INFINITY, lt = 0.f;
+#pragma unroll 4
                     for (uint32_t i = 0; i < parts; ++i) mt = fmaxf(mt, __ldcg(part(i) + kTlItem * DH + rr));
+#pragma unroll 4
                     for (uint32_t i = 0; i < parts; ++i) {
                         const float mi2 = __ldcg(part(i) + kTlItem * DH + rr);
-                        if (mi2 != -INFINITY) lt = fmaf(__ldcg(part(i) + kTlItem * DH + kTlItem + rr), fast_exp2(mi2 - mt), lt);
+                        const float li = __ldcg(part(i) + kTlItem * DH + kTlItem + rr);
+                        lt = fmaf(li, mi2 == -INFINITY ? 0.f : fast_exp2(mi2 - mt), lt);
                     }
                     const float inv = lt == 0.f ? 0.f : 1.f / lt;
-#pragma unroll 1
-                    for (int c = 0; c < DH / 32; ++c) {
-                        float y[32];
+                    float f[4];      // factors of the first parts; more are rare
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) y[i] = 0.f;
-                        for (uint32_t p = 0; p < parts; ++p) {
+                    for (uint32_t p = 0; p < 4; ++p) {
+                        const float mp = p < parts ? __ldcg(part(p) + kTlItem * DH + rr) : -INFINITY;
+                        f[p] = mp == -INFINITY ? 0.f : fast_exp2(mp - mt);
+                    }
+#pragma unroll 2
+                    for (int c = 0; c < (int)kHalfCols / 16; ++c) {
+                        float y[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) y[i] = 0.f;
+                        const size_t at = (size_t)(half * kHalfCols + c * 16) * kTlItem + rr;
+#pragma unroll
+                        for (uint32_t p = 0; p < 4; ++p) {
+                            if (p >= parts) continue;
+                            const float *src = part(p) + at;
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) y[i] = fmaf(__ldcg(src + i * kTlItem), f[p], y[i]);
+                        }
+                        for (uint32_t p = 4; p < parts; ++p) {
                             const float mp = __ldcg(part(p) + kTlItem * DH + rr);
-                            const float f = mp == -INFINITY ? 0.f : fast_exp2(mp - mt);
+                            const float fp = mp == -INFINITY ? 0.f : fast_exp2(mp - mt);
+                            const float *src = part(p) + at;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                y[i] = fmaf(__ldcg(part(p) + (size_t)(c * 32 + i) * kTlItem + rr), f, y[i]);
+                            for (int i = 0; i < 16; ++i) y[i] = fmaf(__ldcg(src + i * kTlItem), fp, y[i]);
                         }
                         write_out(y, c, inv);
                     }
@@ -1147,8 +1195,14 @@ cudaError_t launch_tiles(KvArgs &a, const CUtensorMap &mk, const CUtensorMap &mv
     static_assert(kCounterBytes + (size_t)2 * kMaxSms * kTlItem * (DH + 2) * 4 <= SH_CUDA_KV8_WS_BYTES,
                   "workspace: two partial items per CTA");
     auto kernel = k_attn_kv8_tiles<DH, FP8>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TilesSmem<DH>::kBytes);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TilesSmem<DH>::kBytes);
     if (e != cudaSuccess) return e;
+    // the kernel hands registers from warp to warp: it has to start with as many as it ends with
+    static_assert(512 * kTlRegs + (kTlThreads - 512) * kTlRegsOther <= kTlThreads * 80, "registers");
+    cudaFuncAttributes at;
+    e = cudaFuncGetAttributes(&at, kernel);
+    if (e != cudaSuccess) return e;
+    if (at.numRegs < 80) return cudaErrorInvalidDeviceFunction;
     return sh::launch_pdl(kernel, dim3(sms), dim3(kTlThreads), TilesSmem<DH>::kBytes, st, mk, mv, a);
 }
 
