@@ -5,7 +5,9 @@
 //     o = (sum_j w_j vcode_j) / (sum_j w_j / vs_j)
 // so the value scales ride in the exponent: w_j stays in fp16's range whatever the scales are, and the codes themselves
 // (int8 and e4m3 are exact in fp16) are the operands of the second product. The first product is exact up to its
-// fp32 sums; w_j is rounded to fp16 (2^-11 relative, as the outputs are), its sum is taken in fp32 before that.
+// fp32 sums. The sum of the weights is taken in fp32; for the second product they are fp16 operands, in the kernel for few
+// rows with the rest of that rounding as a second operand (the outputs' own rounding is then all there is; it costs 5 of the
+// 114 us of a large batch), in the one for many rows without it (2^-11 relative, as the outputs' own).
 #include <math.h>
 
 #include "sh_kv8.cuh"
@@ -127,11 +129,12 @@ __device__ __forceinline__ uint32_t byte_pair(uint32_t a, uint32_t b) {
 // both operands agree: a lane takes 16 neighbouring columns of its K rows, and 4 tokens of V with dh / 8 neighbouring
 // columns. W^T comes from S^T by an 8 x 8 transpose in registers.
 //
-// A warp takes 16 tokens of a unit; its K and V boxes (16 rows, swizzled so that neither operand's reads meet in a bank
-// more than two at a time) come by TMA into a ring of its own, kStages ahead and across items, so a warp waits for
-// nobody but its own copies until an item ends. What bounds it beside the bytes is the integer pipe: turning int8 codes
-// into fp16 operands takes 112 of its instructions per 16 tokens and warp at dh = 128, 56 of the 157 cycles that their bytes
-// take, and the rest of a step as much again. The copies alone (no products) run at 0.87 of the measured copy rate.
+// A warp takes 16 tokens of a unit at dh = 128, 32 at dh = 64 (as many bytes); its K and V boxes (16 rows, swizzled so that
+// neither operand's reads meet in a bank more than two at a time) come by TMA into a ring of its own, kStages ahead and
+// across items, so a warp waits for nobody but its own copies until an item ends. What bounds it beside the bytes is the
+// integer pipe: turning int8 codes into fp16 operands takes 112 of its instructions per 16 tokens and warp at dh = 128, 56 of
+// the 157 cycles that their bytes take, and the rest of a step as much again. The copies alone (no products) run at 0.87 of
+// the measured copy rate.
 //
 // Work is split evenly whatever the lengths are: the units (request, kv head, row tile, block of tokens), in this order,
 // are dealt to the CTAs in equal contiguous runs, which every CTA works out from the lengths by itself. An item (request,
@@ -175,10 +178,11 @@ __device__ __forceinline__ void cursor_next(Cursor &k, const KvArgs &a) {
 
 template <int DH, int NT, int NW>
 struct RowsSmem {
-    static constexpr uint32_t kTile = 16 * DH;                        // one K or V box
+    static constexpr uint32_t kTokens = 2048 / DH;                    // of a step: 16 or 32
+    static constexpr uint32_t kTile = kTokens * DH;                   // K or V of a step
     static constexpr uint32_t kRing = 0, kO = NW * kStages * 2 * kTile, kM = kO + NW * 8 * NT * (DH + 4) * 4;
-    static constexpr uint32_t kL = kM + NW * 8 * NT * 4, kScale = kL + NW * 8 * NT * 4;     // ks, vs, in use
-    static constexpr uint32_t kBars = kScale + NW * kStages * 16, kPart = kBars + NW * kStages * 8;
+    static constexpr uint32_t kL = kM + NW * 8 * NT * 4, kScale = kL + NW * 8 * NT * 4;     // {ks, vs, usable} per 16 tokens
+    static constexpr uint32_t kBars = kScale + NW * kStages * 32, kPart = kBars + NW * kStages * 8;
     static constexpr uint32_t kMisc = kPart + NW * 8, kBytes = kMisc + 64 + 1024;
 };
 
@@ -186,7 +190,7 @@ template <int DH, int NT, int NW, bool FP8>
 __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
     k_attn_kv8_rows(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, KvArgs a) {
     using SM = RowsSmem<DH, NT, NW>;
-    constexpr uint32_t RT = 8 * NT, kThreads = NW * 32, kKeys = 16 * NW;      // rows of a tile, keys per unit
+    constexpr uint32_t RT = 8 * NT, kThreads = NW * 32, kStep = SM::kTokens, kKeys = kStep * NW;      // rows of a tile, keys per unit
     constexpr int KC = DH / 64;                     // 16-byte pieces of a K row per lane
     constexpr int VB = DH / 8;                      // V columns per lane
     constexpr int VW = VB / 4;                      // as words
@@ -262,7 +266,7 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
     // ---- the copies run ahead of the sums: cursor `p`. Lane i holds the page of the unit that is i units further in p's item
     // than `p_base`; the table is read again, a step before it is needed, when the item or the 32 units end. -----------
     const uint32_t ring = smem_u32(sm) + SM::kRing + warp * (kStages * 2 * SM::kTile);
-    uint8_t *s_scale = sm + SM::kScale + warp * (kStages * 16);
+    uint8_t *s_scale = sm + SM::kScale + warp * (kStages * 32);
     Cursor k;
     k.r = s_start.r, k.v = s_start.v;
     cursor_sizes<RT, kKeys>(k, a);
@@ -273,14 +277,18 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
     cursor_item<RT, kKeys>(k, a);
     Cursor p = k;
     u64 p_left = end - begin;
-    // the warp's 16 tokens of the cursor's unit hold keys
-    auto in_use = [&](const Cursor &x) { return (int)(x.b * kKeys + warp * 16) < x.lim_hi; };
+    // the warp's tokens of the cursor's unit hold keys
+    auto in_use = [&](const Cursor &x) { return (int)(x.b * kKeys + warp * kStep) < x.lim_hi; };
+    constexpr int HF = kStep / 16;      // groups of 16 tokens, each in one page
     uint32_t p_base = k.b;
-    int p_ids = -1;
+    int p_ids[HF];
     auto lookup = [&]() {
         p_base = p.b;
-        const uint32_t tok = (p.b + lane) * kKeys + warp * 16;
-        p_ids = p_left && (int)tok < p.lim_hi ? a.table[(size_t)p.r * a.ld_table + (tok >> a.page_shift)] : -1;
+#pragma unroll
+        for (int f = 0; f < HF; ++f) {
+            const uint32_t tok = (p.b + lane) * kKeys + warp * kStep + f * 16;
+            p_ids[f] = p_left && (int)tok < p.lim_hi ? a.table[(size_t)p.r * a.ld_table + (tok >> a.page_shift)] : -1;
+        }
     };
     lookup();
     auto advance = [&]() {
@@ -292,25 +300,35 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
     auto issue = [&]() {      // the next unit in which this warp has keys
         while (p_left && !in_use(p)) advance();
         if (p_left == 0) return;
-        const int p_id = __shfl_sync(0xffffffffu, p_ids, p.b - p_base);
+        int id[HF];
+#pragma unroll
+        for (int f = 0; f < HF; ++f) id[f] = __shfl_sync(0xffffffffu, p_ids[f], p.b - p_base);
         if (lane == 0) {
-            int *info = reinterpret_cast<int *>(s_scale + p_slot * 16);
-            const bool good = (uint32_t)p_id < a.pages;
-            info[2] = good;
-            if (good) {
-                const int row = (int)((p.kvh << a.page_shift) + ((p.b * kKeys + warp * 16) & page1));
-                uint8_t *dst = sm + SM::kRing + (warp * kStages + p_slot) * (2 * SM::kTile);
-                mbar_arrive_expect_tx(full + p_slot, 2 * SM::kTile);
-                tma_load_3d(dst, &mk, full + p_slot, 0, row, p_id);
-                tma_load_3d(dst + SM::kTile, &mv, full + p_slot, 0, row, p_id);
-                cp_async4(smem_u32(info), a.ks + (size_t)p_id * a.heads + p.kvh);
-                cp_async4(smem_u32(info) + 4, a.vs + (size_t)p_id * a.heads + p.kvh);
-                cp_async_arrive(full + p_slot);
-            } else {
-                atomicCAS(a.err, 0, (int)sh::kErrBadArgs);
-                mbar_arrive(full + p_slot);
-                mbar_arrive(full + p_slot);
+            constexpr uint32_t kBox = SM::kTile / HF;
+            const uint32_t tok = p.b * kKeys + warp * kStep;
+            uint64_t *bar = full + p_slot;
+            uint8_t *dst = sm + SM::kRing + (warp * kStages + p_slot) * (2 * SM::kTile);
+            int *info = reinterpret_cast<int *>(s_scale + p_slot * 32);
+            uint32_t boxes = 0;
+#pragma unroll
+            for (int f = 0; f < HF; ++f) boxes += (uint32_t)id[f] < a.pages;
+            mbar_arrive_expect_tx(bar, boxes * 2 * kBox);
+#pragma unroll
+            for (int f = 0; f < HF; ++f) {
+                const bool good = (uint32_t)id[f] < a.pages;
+                info[4 * f + 2] = good;
+                if (good) {
+                    const int row = (int)((p.kvh << a.page_shift) + ((tok + f * 16) & page1));
+                    const size_t at = (size_t)id[f] * a.heads + p.kvh;
+                    tma_load_3d(dst + f * kBox, &mk, bar, 0, row, id[f]);
+                    tma_load_3d(dst + SM::kTile + f * kBox, &mv, bar, 0, row, id[f]);
+                    cp_async4(smem_u32(info + 4 * f), a.ks + at);
+                    cp_async4(smem_u32(info + 4 * f) + 4, a.vs + at);
+                } else if ((int)tok + f * 16 < p.lim_hi) {
+                    atomicCAS(a.err, 0, (int)sh::kErrBadArgs);
+                }
             }
+            cp_async_arrive(bar);
         }
         p_slot = p_slot + 1 == kStages ? 0 : p_slot + 1;
         advance();
@@ -373,117 +391,124 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
         for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = l[nt][0] = l[nt][1] = 0.f, top[nt][0] = top[nt][1] = -INFINITY;
 
         for (uint32_t b = b0; b < b1; ++b) {
-            const int tok0 = (int)(b * kKeys + warp * 16);
-            if (tok0 >= lim_hi) break;
+            if ((int)(b * kKeys + warp * kStep) >= lim_hi) break;
             if (!mbar_try_wait(full + slot, phase)) mbar_wait(full + slot, phase, abort, a.err);
-            const uint32_t kt = ring + slot * (2 * SM::kTile), vt = kt + SM::kTile;
-            const float *info = reinterpret_cast<const float *>(s_scale + slot * 16);
+            const uint32_t ring_at = ring + slot * (2 * SM::kTile);
+            const uint8_t *infos = s_scale + slot * 32;
             slot = slot + 1 == kStages ? 0 : slot + 1;
             phase ^= slot == 0;
-            const float ks = info[0], vs = info[1];
-            if (reinterpret_cast<const int *>(info)[2] == 0) {      // no such page: these tokens are left out
-                __syncwarp();
-                issue();
-                continue;
-            }
-            float s[NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+            for (int f = 0; f < HF; ++f) {
+                const int tok0 = (int)(b * kKeys + warp * kStep + f * 16);
+                const float4 info = *reinterpret_cast<const float4 *>(infos + 16 * f);
+                if (__float_as_int(info.z) == 0) continue;      // no keys of this tile, or no such page: left out
+                const uint32_t kt = ring_at + f * 16 * DH, vt = kt + SM::kTile;
+                const float ks = info.x, vs = info.y;
+                float s[NT][4];
 #pragma unroll
-            for (int j = 0; j < KC; ++j) {
-                // rows g and g + 8, columns 64 j + 16 c ..: 128-byte rows have piece x at x ^ (row % 8), 64-byte rows at
-                // x ^ (row / 2 % 4)
-                const uint32_t at = kt + g * DH + (DH == 128 ? ((j * 4 + c) ^ g) * 16 : (c ^ (g >> 1)) * 16);
-                const uint4 ka4 = lds16(at), kb4 = lds16(at + 8 * DH);
-                const uint32_t ka[4] = {ka4.x, ka4.y, ka4.z, ka4.w}, kb[4] = {kb4.x, kb4.y, kb4.z, kb4.w};
+                for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t a0, a1, a2, a3;
-                    word_to_h2<FP8>(ka[i], a0, a2);
-                    word_to_h2<FP8>(kb[i], a1, a3);
+                for (int j = 0; j < KC; ++j) {
+                    // rows g and g + 8, columns 64 j + 16 c ..: 128-byte rows have piece x at x ^ (row % 8), 64-byte rows at
+                    // x ^ (row / 2 % 4)
+                    const uint32_t at = kt + g * DH + (DH == 128 ? ((j * 4 + c) ^ g) * 16 : (c ^ (g >> 1)) * 16);
+                    const uint4 ka4 = lds16(at), kb4 = lds16(at + 8 * DH);
+                    const uint32_t ka[4] = {ka4.x, ka4.y, ka4.z, ka4.w}, kb[4] = {kb4.x, kb4.y, kb4.z, kb4.w};
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        mma16816(s[nt], a0, a1, a2, a3, qf[nt][j * 4 + i][0], qf[nt][j * 4 + i][1]);
-                }
-            }
-            const float ksl = ks * a.sl2, vcl = fmaxf(vs, 0x1p-80f);
-            {
-                const float lvs = __log2f(vcl), rvs = __frcp_rn(vcl);
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t a0, a1, a2, a3;
+                        word_to_h2<FP8>(ka[i], a0, a2);
+                        word_to_h2<FP8>(kb[i], a1, a3);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[nt][e] = fmaf(s[nt][e], ksl, lvs);
-                if (tok0 + 16 > lim_lo) {
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (tok0 + (int)g + 8 * (e >> 1) >= lim[nt][e & 1]) s[nt][e] = -INFINITY;
-                }
-                bool raise = false;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) raise |= fmaxf(s[nt][e], s[nt][e + 2]) > top[nt][e];
-                // the maximum only moves when a weight would pass 2^8 (exact room in fp16), which is rare after the start
-                if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float x = fmaxf(s[nt][e], s[nt][e + 2]);
-#pragma unroll
-                            for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                            const float was = top[nt][e] - 8.f, now = fmaxf(was, x);
-                            const float f = now == -INFINITY ? 1.f : fast_exp2(was - now);
-                            top[nt][e] = now + 8.f;
-                            m[nt][e] = now == -INFINITY ? 0.f : now;
-                            l[nt][e] *= f;
-#pragma unroll
-                            for (int i = 0; i < DH / 16; ++i) o[i][nt][e] *= f, o[i][nt][e + 2] *= f;
-                        }
-                }
-                uint32_t w0[NT], w1[NT];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        w[e] = fast_exp2(s[nt][e] - m[nt][e & 1]);
-                        l[nt][e & 1] = fmaf(w[e], rvs, l[nt][e & 1]);
-                    }
-                    w0[nt] = movmatrix(pack_h2(w[0], w[1]));
-                    w1[nt] = movmatrix(pack_h2(w[2], w[3]));
-                }
-                uint32_t vr[4][VW];      // tokens 2 c, 2 c + 1, 2 c + 8, 2 c + 9, columns VB g ..
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t tok = 2 * c + (e & 1) + 8 * (e >> 1);
-                    if (VW == 4) {
-                        const uint4 x = lds16(vt + tok * DH + (g ^ (tok & 7)) * 16);
-                        vr[e][0] = x.x, vr[e][1] = x.y, vr[e][VW - 2] = x.z, vr[e][VW - 1] = x.w;
-                    } else {
-                        const uint2 x = lds8(vt + tok * DH + ((g >> 1) ^ (tok >> 1 & 3)) * 16 + (g & 1) * 8);
-                        vr[e][0] = x.x, vr[e][1] = x.y;
+                        for (int nt = 0; nt < NT; ++nt)
+                            mma16816(s[nt], a0, a1, a2, a3, qf[nt][j * 4 + i][0], qf[nt][j * 4 + i][1]);
                     }
                 }
-                if (tok0 + 16 > lim_hi) {      // rows that are no keys can hold anything
+                const float ksl = ks * a.sl2, vcl = fmaxf(vs, 0x1p-80f);
+                {
+                    const float lvs = __log2f(vcl), rvs = __frcp_rn(vcl);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (tok0 + (int)(2 * c + (e & 1) + 8 * (e >> 1)) >= lim_hi)
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                            for (int i = 0; i < VW; ++i) vr[e][i] = 0;
-                }
+                        for (int e = 0; e < 4; ++e) s[nt][e] = fmaf(s[nt][e], ksl, lvs);
+                    if (tok0 + 16 > lim_lo) {
 #pragma unroll
-                for (int i = 0; i < VW; ++i) {
-                    const uint32_t a00 = byte_pair<FP8, 0>(vr[0][i], vr[1][i]), a02 = byte_pair<FP8, 0>(vr[2][i], vr[3][i]);
-                    const uint32_t a01 = byte_pair<FP8, 1>(vr[0][i], vr[1][i]), a03 = byte_pair<FP8, 1>(vr[2][i], vr[3][i]);
-                    const uint32_t a10 = byte_pair<FP8, 2>(vr[0][i], vr[1][i]), a12 = byte_pair<FP8, 2>(vr[2][i], vr[3][i]);
-                    const uint32_t a11 = byte_pair<FP8, 3>(vr[0][i], vr[1][i]), a13 = byte_pair<FP8, 3>(vr[2][i], vr[3][i]);
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (tok0 + (int)g + 8 * (e >> 1) >= lim[nt][e & 1]) s[nt][e] = -INFINITY;
+                    }
+                    bool raise = false;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) raise |= fmaxf(s[nt][e], s[nt][e + 2]) > top[nt][e];
+                    // the maximum only moves when a weight would pass 2^8 (exact room in fp16), which is rare after the start
+                    if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                float x = fmaxf(s[nt][e], s[nt][e + 2]);
+#pragma unroll
+                                for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                                const float was = top[nt][e] - 8.f, now = fmaxf(was, x);
+                                const float f = now == -INFINITY ? 1.f : fast_exp2(was - now);
+                                top[nt][e] = now + 8.f;
+                                m[nt][e] = now == -INFINITY ? 0.f : now;
+                                l[nt][e] *= f;
+#pragma unroll
+                                for (int i = 0; i < DH / 16; ++i) o[i][nt][e] *= f, o[i][nt][e + 2] *= f;
+                            }
+                    }
+                    uint32_t w0[NT], w1[NT], d0[NT], d1[NT];      // weights in fp16, and what that rounding left
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        mma16816(o[2 * i][nt], a00, a01, a02, a03, w0[nt], w1[nt]);
-                        mma16816(o[2 * i + 1][nt], a10, a11, a12, a13, w0[nt], w1[nt]);
+                        float w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            w[e] = fast_exp2(s[nt][e] - m[nt][e & 1]);
+                            l[nt][e & 1] = fmaf(w[e], rvs, l[nt][e & 1]);
+                        }
+                        const __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
+                        const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+                        w0[nt] = movmatrix(*reinterpret_cast<const uint32_t *>(&h0));
+                        w1[nt] = movmatrix(*reinterpret_cast<const uint32_t *>(&h1));
+                        d0[nt] = movmatrix(pack_h2(w[0] - f0.x, w[1] - f0.y));
+                        d1[nt] = movmatrix(pack_h2(w[2] - f1.x, w[3] - f1.y));
+                    }
+                    uint32_t vr[4][VW];      // tokens 2 c, 2 c + 1, 2 c + 8, 2 c + 9, columns VB g ..
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t tok = 2 * c + (e & 1) + 8 * (e >> 1);
+                        if (VW == 4) {
+                            const uint4 x = lds16(vt + tok * DH + (g ^ (tok & 7)) * 16);
+                            vr[e][0] = x.x, vr[e][1] = x.y, vr[e][VW - 2] = x.z, vr[e][VW - 1] = x.w;
+                        } else {
+                            const uint2 x = lds8(vt + tok * DH + ((g >> 1) ^ (tok >> 1 & 3)) * 16 + (g & 1) * 8);
+                            vr[e][0] = x.x, vr[e][1] = x.y;
+                        }
+                    }
+                    if (tok0 + 16 > lim_hi) {      // rows that are no keys can hold anything
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (tok0 + (int)(2 * c + (e & 1) + 8 * (e >> 1)) >= lim_hi)
+#pragma unroll
+                                for (int i = 0; i < VW; ++i) vr[e][i] = 0;
+                    }
+#pragma unroll
+                    for (int i = 0; i < VW; ++i) {
+                        const uint32_t a00 = byte_pair<FP8, 0>(vr[0][i], vr[1][i]), a02 = byte_pair<FP8, 0>(vr[2][i], vr[3][i]);
+                        const uint32_t a01 = byte_pair<FP8, 1>(vr[0][i], vr[1][i]), a03 = byte_pair<FP8, 1>(vr[2][i], vr[3][i]);
+                        const uint32_t a10 = byte_pair<FP8, 2>(vr[0][i], vr[1][i]), a12 = byte_pair<FP8, 2>(vr[2][i], vr[3][i]);
+                        const uint32_t a11 = byte_pair<FP8, 3>(vr[0][i], vr[1][i]), a13 = byte_pair<FP8, 3>(vr[2][i], vr[3][i]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma16816(o[2 * i][nt], a00, a01, a02, a03, w0[nt], w1[nt]);
+                            mma16816(o[2 * i + 1][nt], a10, a11, a12, a13, w0[nt], w1[nt]);
+                            mma16816(o[2 * i][nt], a00, a01, a02, a03, d0[nt], d1[nt]);
+                            mma16816(o[2 * i + 1][nt], a10, a11, a12, a13, d0[nt], d1[nt]);
+                        }
                     }
                 }
             }

@@ -76,6 +76,7 @@ __device__ __forceinline__ Req request(int len, int add, uint32_t shift, uint32_
     return q;
 }
 
+template <uint32_t PER>
 __global__ void __launch_bounds__(kTabThreads) k_kv_tables(TablesArgs a) {
     extern __shared__ uint32_t sm[];
     __shared__ uint32_t part[kTabThreads / 32][3];
@@ -110,15 +111,21 @@ __global__ void __launch_bounds__(kTabThreads) k_kv_tables(TablesArgs a) {
     __syncthreads();
     if (t == 0 && gridDim.x > 1) s_last = atom_add_acq_rel_gpu(a.pool_out + 7, 1u) == gridDim.x - 1;
 
-    // ---- the slot map: four neighbouring tokens per thread (new table entries also of tokens past t_cap) ---------------
+    // ---- the slot map: PER neighbouring tokens per thread, their look-ups in flight together (new table entries also of
+    // tokens past t_cap) ------------------------------------------------------------------------------------------------
     const uint32_t page1 = (1u << a.page_shift) - 1, total = s_tok[R - 1], stop = max(total, a.t_cap);
-    for (uint64_t i0 = 4ull * ((uint64_t)blockIdx.x * kTabThreads + t); i0 < stop; i0 += 4ull * gridDim.x * kTabThreads) {
-        int slot[4], pos[4];
+    auto wrap = [&](uint32_t i) { return i < a.pages ? i : i - a.pages; };      // i < 2 pages
+    for (uint64_t i0 = (uint64_t)PER * ((uint64_t)blockIdx.x * kTabThreads + t); i0 < stop;
+         i0 += (uint64_t)PER * gridDim.x * kTabThreads) {
+        int slot[PER], pos[PER];
+        int *entry[PER];            // the token's table entry, to be written when its page is new and the token is its first
+        const int *from[PER];       // where the page's id is
+        bool fresh[PER];
         uint32_t r = upper_bound(s_tok, R, (uint32_t)i0);
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
+        for (uint32_t j = 0; j < PER; ++j) {
             const uint32_t i = (uint32_t)i0 + j;
-            slot[j] = -1, pos[j] = 0;
+            slot[j] = -1, pos[j] = 0, from[j] = nullptr, entry[j] = nullptr, fresh[j] = false;
             if (i >= total) continue;
             while (r < R - 1 && s_tok[r] <= i) ++r;
             const uint32_t before = r ? s_tok[r - 1] : 0u, nb = r ? s_need[r - 1] : 0u, len = s_len[r];
@@ -127,27 +134,44 @@ __global__ void __launch_bounds__(kTabThreads) k_kv_tables(TablesArgs a) {
             pos[j] = (int)p;
             const bool fits = (((uint64_t)len + n + page1) >> a.page_shift) <= a.ld_table;
             if (!fits || b >= a.ld_table || (need_r && s_need[r] > count)) continue;   // put off
-            uint32_t pid;
-            if (b < have)
-                pid = (uint32_t)a.table[(size_t)r * a.ld_table + b];
-            else {
-                pid = (uint32_t)a.ring[(head + nb + (b - have)) % a.pages];
-                if ((p & page1) == 0) a.table[(size_t)r * a.ld_table + b] = (int)pid;
-            }
-            slot[j] = (int)((pid << a.page_shift) + (p & page1));
+            entry[j] = a.table + (size_t)r * a.ld_table + b;
+            fresh[j] = b >= have;
+            from[j] = fresh[j] ? a.ring + wrap(head + min(nb + (b - have), a.pages - 1)) : entry[j];
         }
-        if (a.vec && i0 + 4 <= a.t_cap) {
-            *reinterpret_cast<int4 *>(a.slots + i0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
-            *reinterpret_cast<int4 *>(a.pos + i0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+        int pid[PER];
+#pragma unroll
+        for (uint32_t j = 0; j < PER; ++j) pid[j] = from[j] ? *from[j] : 0;
+#pragma unroll
+        for (uint32_t j = 0; j < PER; ++j) {
+            const uint32_t in = (uint32_t)pos[j] & page1;
+            if (from[j]) slot[j] = (int)(((uint32_t)pid[j] << a.page_shift) + in);
+            if (fresh[j] && in == 0) *entry[j] = pid[j];
+        }
+        if (PER == 4 && a.vec && i0 + PER <= a.t_cap) {
+            *reinterpret_cast<int4 *>(a.slots + i0) = make_int4(slot[0], slot[PER > 1 ? 1 : 0], slot[PER > 2 ? 2 : 0], slot[PER - 1]);
+            *reinterpret_cast<int4 *>(a.pos + i0) = make_int4(pos[0], pos[PER > 1 ? 1 : 0], pos[PER > 2 ? 2 : 0], pos[PER - 1]);
         } else {
-            for (uint32_t j = 0; j < 4 && i0 + j < a.t_cap; ++j) a.slots[i0 + j] = slot[j], a.pos[i0 + j] = pos[j];
+#pragma unroll
+            for (uint32_t j = 0; j < PER; ++j)
+                if (i0 + j < a.t_cap) a.slots[i0 + j] = slot[j], a.pos[i0 + j] = pos[j];
         }
     }
-    // ---- pages given back ------------------------------------------------------------------------------------------
-    const uint32_t gone = s_back[R - 1];
-    for (uint64_t i = (uint64_t)blockIdx.x * kTabThreads + t; i < gone; i += (uint64_t)gridDim.x * kTabThreads) {
-        const uint32_t r = upper_bound(s_back, R, (uint32_t)i), before = r ? s_back[r - 1] : 0u;
-        a.ring[((uint64_t)head + count + i) % a.pages] = a.table[(size_t)r * a.ld_table + ((uint32_t)i - before)];
+    // ---- pages given back, four look-ups of a thread in flight --------------------------------------------------------
+    const uint32_t gone = s_back[R - 1], step = gridDim.x * kTabThreads;
+    for (uint64_t i0 = (uint64_t)blockIdx.x * kTabThreads + t; i0 < gone; i0 += 4ull * step) {
+        int id[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            const uint64_t i = i0 + (uint64_t)j * step;
+            if (i >= gone) continue;
+            const uint32_t r = upper_bound(s_back, R, (uint32_t)i), before = r ? s_back[r - 1] : 0u;
+            id[j] = a.table[(size_t)r * a.ld_table + ((uint32_t)i - before)];
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            const uint64_t i = i0 + (uint64_t)j * step;
+            if (i < gone) a.ring[((uint64_t)head + count + i) % a.pages] = id[j];
+        }
     }
     // ---- the new state: by the CTA that was the last to read the old one ---------------------------------------------
     __syncthreads();
@@ -180,8 +204,9 @@ __global__ void __launch_bounds__(kTabThreads) k_kv_tables(TablesArgs a) {
 // Append. The scale of a page and head covers all of its tokens, so the new tokens of a page are handled by one
 // CTA per head and per K / V: the CTA of the page's first new token (its "leader"). A CTA owns `chunk` rows of the slot
 // map and takes the pages whose leader is among them, reading on past its rows to the end of the last such page. Phases:
-// runs of one page from the slots, max |x| per run (rows read once from HBM), the new scale, codes (rows read again from
-// L1 / L2), older codes of pages whose scale grew. DH / 8 lanes hold a row, 16 bytes each.
+// runs of one page from the slots, max |x| per run (rows read once from HBM), the new scale, codes (rows still in
+// registers, or again from L2 when there are more than a batch), older codes of pages whose scale grew. DH / 8 lanes hold a
+// row, 16 bytes each.
 // Bound by HBM for prompts (6 bytes per element) and by latency for single tokens.
 // ================================================================================================================
 constexpr uint32_t kAppThreads = 256, kAppWin = 256 + 1;
@@ -197,21 +222,28 @@ struct AppendArgs {
     int *err;
 };
 
-__device__ __forceinline__ float clean(__half h) {   // NaN -> 0, infinities -> the largest fp16
-    const float x = __half2float(h);
-    return isnan(x) ? 0.f : fminf(fmaxf(x, -65504.f), 65504.f);
-}
 // the next fp32 value with 8 significant bits, for x >= 0
 __device__ __forceinline__ float up8(float x) { return __uint_as_float((__float_as_uint(x) + 0xFFFFu) & ~0xFFFFu); }
 
+// x / s, correctly rounded, from r = 1 / s (correctly rounded): the remainder is exact, so a quotient that is representable
+// (a border between two codes, which has at most 9 bits) comes out as it is. No operand here is near over- or underflow.
+__device__ __forceinline__ float divide(float x, float s, float r) {
+    const float q = x * r;
+    return fmaf(fmaf(-q, s, x), r, q);
+}
+// the codes of four quotients, |y| <= qmax
 template <bool FP8>
-__device__ __forceinline__ uint32_t encode(float y) {   // |y| <= qmax up to rounding
+__device__ __forceinline__ uint32_t encode4(float y0, float y1, float y2, float y3) {
     if (FP8) {
-        uint16_t r;
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(y));
-        return r & 0xFFu;
+        uint16_t lo, hi;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y1), "f"(y0));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y3), "f"(y2));
+        return (uint32_t)lo | (uint32_t)hi << 16;
     }
-    return (uint32_t)min(max(__float2int_rn(y), -127), 127) & 0xFFu;
+    // adding 1.5 2^23 rounds to a whole number, to nearest even, and leaves its two's complement in the low byte
+    const uint32_t a = __float_as_uint(y0 + 12582912.f), b = __float_as_uint(y1 + 12582912.f);
+    const uint32_t c = __float_as_uint(y2 + 12582912.f), d = __float_as_uint(y3 + 12582912.f);
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 template <bool FP8>
 __device__ __forceinline__ float decode(uint32_t c) {
@@ -223,17 +255,43 @@ __device__ __forceinline__ float decode(uint32_t c) {
     return (float)(int8_t)c;
 }
 
-template <int DH, bool VEC>
-__device__ __forceinline__ void load_row8(float (&f)[8], const __half *row, uint32_t l) {
-    __half h[8];
+// 8 fp16 values of a row
+template <bool VEC>
+__device__ __forceinline__ void raw8(uint32_t (&w)[4], const __half *p) {
     if (VEC) {
-        *reinterpret_cast<uint4 *>(h) = *reinterpret_cast<const uint4 *>(row + l * 8);
+        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) h[j] = row[l * 8 + j];
+        for (int j = 0; j < 4; ++j)
+            w[j] = (uint32_t)__half_as_ushort(p[2 * j]) | (uint32_t)__half_as_ushort(p[2 * j + 1]) << 16;
     }
+}
+// NaN becomes 0 and infinities the largest fp16; returns the largest magnitude
+__device__ __forceinline__ float clean8(uint32_t (&w)[4]) {
+    auto largest = [&]() {
+        __half2 m = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = clean(h[j]);
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t abs2 = w[j] & 0x7FFF7FFFu;
+            m = __hmax2_nan(m, *reinterpret_cast<const __half2 *>(&abs2));
+        }
+        return __half2float(__hmax_nan(__low2half(m), __high2half(m)));
+    };
+    float m = largest();
+    if (!(m <= 65504.f)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t h = w[j] >> (16 * e) & 0xFFFFu;
+                if ((h & 0x7C00u) != 0x7C00u) continue;
+                const uint32_t to = h & 0x3FFu ? 0u : (h & 0x8000u) | 0x7BFFu;
+                w[j] = (w[j] & ~(0xFFFFu << (16 * e))) | to << (16 * e);
+            }
+        m = largest();
+    }
+    return m;
 }
 
 template <int DH, bool FP8, bool VEC>
@@ -245,7 +303,8 @@ __global__ void __launch_bounds__(kAppThreads) k_kv8_append(AppendArgs a) {
     __shared__ uint32_t s_amax[kAppWin], s_min[kAppWin];
     __shared__ float s_old[kAppWin], s_new[kAppWin];
     __shared__ int s_lead[kAppThreads / 32];
-    __shared__ uint32_t s_end;
+    __shared__ uint32_t s_end, s_grown_n;
+    __shared__ uint8_t s_grown[kAppThreads];       // leaders whose page's scale grew over older rows, as window index - 1
     pdl_launch_dependents();
     pdl_wait();
     const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -254,7 +313,7 @@ __global__ void __launch_bounds__(kAppThreads) k_kv8_append(AppendArgs a) {
     const int last_slot = (int)(a.pages << a.page_shift);
     // window index 0 is the row before the chunk
     for (uint32_t j = t; j <= win; j += kAppThreads) s_slot[j] = first + j == 0 ? -1 : a.slots[first + j - 1];
-    if (t == 0) s_end = 0;
+    if (t == 0) s_end = 0, s_grown_n = 0;
     __syncthreads();
 
     // a leader is a valid row whose predecessor is not of the same page
@@ -300,19 +359,33 @@ __global__ void __launch_bounds__(kAppThreads) k_kv8_append(AppendArgs a) {
 
     const __half *x = (kv ? a.x[1] : a.x[0]) + (size_t)h * DH;
     const uint32_t ld = kv ? a.ld[1] : a.ld[0], l = t % LPR, rw = t / LPR;
-    for (uint32_t r = 1; r < end; r += kRows) {    // every lane walks the loop: the reductions are warp-wide
-        const uint32_t i = r + rw;
-        const int run = i < end ? s_run[i] : -1;
-        float m = 0.f;
-        if (run >= 0) {
-            float f[8];
-            load_row8<DH, VEC>(f, x + (size_t)(first + i - 1) * ld, l);
+    // rows of this thread, kBatch at a time so that their loads are in flight together; one batch is held in registers
+    constexpr uint32_t kBatch = 8;
+    uint32_t w[kBatch][4];
+    auto load_batch = [&](uint32_t r0, float (&m)[kBatch]) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(f[e]));
+        for (uint32_t b = 0; b < kBatch; ++b) {
+            const uint32_t i = r0 + b * kRows + rw;
+            m[b] = 0.f;
+            if (i < end && s_run[i] >= 0) raw8<VEC>(w[b], x + (size_t)(first + i - 1) * ld + l * 8);
         }
 #pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (run >= 0 && l == 0) atomicMax(&s_amax[run], __float_as_uint(m));
+        for (uint32_t b = 0; b < kBatch; ++b) {
+            const uint32_t i = r0 + b * kRows + rw;
+            if (i < end && s_run[i] >= 0) m[b] = clean8(w[b]);
+        }
+    };
+    float m[kBatch];
+    for (uint32_t r0 = 1; r0 < end; r0 += kBatch * kRows) {    // every lane walks the loop: the reductions are warp-wide
+        load_batch(r0, m);
+#pragma unroll
+        for (uint32_t b = 0; b < kBatch; ++b) {
+            if (r0 + b * kRows >= end) break;
+#pragma unroll
+            for (int o = LPR / 2; o > 0; o >>= 1) m[b] = fmaxf(m[b], __shfl_xor_sync(0xffffffffu, m[b], o));
+            const uint32_t i = r0 + b * kRows + rw;
+            if (l == 0 && i < end && s_run[i] >= 0) atomicMax(&s_amax[s_run[i]], __float_as_uint(m[b]));
+        }
     }
     __syncthreads();
     float *scale = kv ? a.scale[1] : a.scale[0];
@@ -323,40 +396,48 @@ __global__ void __launch_bounds__(kAppThreads) k_kv8_append(AppendArgs a) {
         s_old[j] = old;
         s_new[j] = now;
         *sp = now;
+        if (s_min[j] && now > old) s_grown[atomicAdd(&s_grown_n, 1u)] = (uint8_t)t;
     }
     __syncthreads();
     uint8_t *codes = kv ? a.codes[1] : a.codes[0];
     const size_t head_off = (size_t)h << a.page_shift;
-    for (uint32_t r = 1; r < end; r += kRows) {
-        const uint32_t i = r + rw;
-        const int run = i < end ? s_run[i] : -1;
-        if (run < 0) continue;
-        const float s = s_new[run];
-        float f[8];
-        load_row8<DH, VEC>(f, x + (size_t)(first + i - 1) * ld, l);
-        uint32_t w[2] = {0, 0};
-        if (s > 0.f) {
+    for (uint32_t r0 = 1; r0 < end; r0 += kBatch * kRows) {
+        if (end > 1 + kBatch * kRows) load_batch(r0, m);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e >> 2] |= encode<FP8>(__fdiv_rn(f[e], s)) << (8 * (e & 3));
+        for (uint32_t b = 0; b < kBatch; ++b) {
+            const uint32_t i = r0 + b * kRows + rw;
+            const int run = i < end ? s_run[i] : -1;
+            if (run < 0) continue;
+            const float s = s_new[run], r1 = s > 0.f ? __frcp_rn(s) : 0.f;      // scale 0: all values are
+            uint32_t c[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float2 a0 = __half22float2(*reinterpret_cast<const __half2 *>(&w[b][2 * e]));
+                const float2 a1 = __half22float2(*reinterpret_cast<const __half2 *>(&w[b][2 * e + 1]));
+                c[e] = encode4<FP8>(divide(a0.x, s, r1), divide(a0.y, s, r1), divide(a1.x, s, r1), divide(a1.y, s, r1));
+            }
+            const uint32_t sl = (uint32_t)s_slot[i];
+            uint8_t *dst = codes + (size_t)(sl >> a.page_shift) * a.page_stride + (head_off + (sl & (page - 1))) * DH + l * 8;
+            *reinterpret_cast<uint2 *>(dst) = make_uint2(c[0], c[1]);
         }
-        const uint32_t sl = (uint32_t)s_slot[i];
-        uint8_t *dst = codes + (size_t)(sl >> a.page_shift) * a.page_stride + (head_off + (sl & (page - 1))) * DH + l * 8;
-        *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
     }
     // older rows of pages whose scale grew: code s / s', rounded once more
-    for (uint32_t q = 1; q <= min(win, a.chunk); ++q) {
-        if (s_run[q] != (int)q || !(s_new[q] > s_old[q])) continue;
-        const float so = s_old[q], sn = s_new[q];
+    for (uint32_t k = 0; k < s_grown_n; ++k) {
+        const uint32_t q = s_grown[k] + 1u;
+        const float so = s_old[q], sn = s_new[q], r1 = __frcp_rn(sn);
         uint8_t *base = codes + (size_t)((uint32_t)s_slot[q] >> a.page_shift) * a.page_stride + head_off * DH;
         for (uint32_t row = rw; row < s_min[q]; row += kRows) {
             uint2 *p = reinterpret_cast<uint2 *>(base + (size_t)row * DH + l * 8);
             const uint2 c = *p;
             const uint32_t cw[2] = {c.x, c.y};
-            uint32_t w[2] = {0, 0};
+            uint32_t w[2];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                w[e >> 2] |= encode<FP8>(__fdiv_rn(decode<FP8>((cw[e >> 2] >> (8 * (e & 3))) & 0xFFu) * so, sn))
-                             << (8 * (e & 3));
+            for (int e = 0; e < 2; ++e) {
+                float y[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] = divide(decode<FP8>(cw[e] >> (8 * j) & 0xFFu) * so, sn, r1);
+                w[e] = encode4<FP8>(y[0], y[1], y[2], y[3]);
+            }
             *p = make_uint2(w[0], w[1]);
         }
     }
@@ -391,15 +472,17 @@ int sh_cuda_kv_tables(uint64_t lens, uint64_t add, uint32_t R, uint32_t page, ui
     TablesArgs a = {(const int *)lens, (const int *)add, (int *)table, (int *)ring, (const uint32_t *)pool,
                     (uint32_t *)pool_out, (int *)lens_out, (int *)q_start, (int *)slots, (int *)pos, R,
                     sh::kv8_shift(page), ld_table, pages, t_cap, sh::aligned16(slots) && sh::aligned16(pos)};
-    const uint32_t want = (t_cap + 4 * kTabThreads - 1) / (4 * kTabThreads), cap = s.num_sms > 0 ? s.num_sms : 1;
-    const uint32_t grid = want < 1 ? 1 : want < cap ? want : cap;
+    // one token per thread while that fills no GPU, four (16-byte stores) beyond
+    const uint32_t cap = s.num_sms > 0 ? s.num_sms : 1, per = t_cap > cap * kTabThreads ? 4 : 1;
+    const uint64_t want = ((uint64_t)t_cap + per * kTabThreads - 1) / (per * kTabThreads);
+    const uint32_t grid = want < 1 ? 1 : want < cap ? (uint32_t)want : cap;
     const size_t smem = (size_t)R * 16;
+    auto kernel = per == 4 ? k_kv_tables<4> : k_kv_tables<1>;
     if (smem > 48 * 1024 &&
-        !sh::cuda_ok(cudaFuncSetAttribute(k_kv_tables, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kTabMaxR * 16)),
+        !sh::cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kTabMaxR * 16)),
                      "sh_cuda_kv_tables"))
         return -1;
-    return sh::cuda_ok(sh::launch_pdl(k_kv_tables, dim3(grid), dim3(kTabThreads), smem, s.stream, a),
-                       "sh_cuda_kv_tables") ? 0 : -1;
+    return sh::cuda_ok(sh::launch_pdl(kernel, dim3(grid), dim3(kTabThreads), smem, s.stream, a), "sh_cuda_kv_tables") ? 0 : -1;
 }
 
 int sh_cuda_kv8_append(const sh_cuda_kv8_t *c, uint64_t k, uint64_t v, uint32_t T, uint32_t ldk, uint32_t ldv,
@@ -417,10 +500,12 @@ int sh_cuda_kv8_append(const sh_cuda_kv8_t *c, uint64_t k, uint64_t v, uint32_t 
     AppendArgs a = {{(uint8_t *)c->k, (uint8_t *)c->v}, {(float *)c->k_scale, (float *)c->v_scale},
                     {(const __half *)k, (const __half *)v}, {ldk, ldv}, (const int *)slots, c->page_stride, T, c->pages,
                     sh::kv8_shift(c->page), c->heads, 0, s.dev_err};
-    // A prompt's pages hold up to `page` new rows each: one page per CTA. Few rows are mostly one per page: eight rows
-    // per CTA spread them over the GPU.
-    const uint64_t ctas = (uint64_t)((T + c->page - 1) / c->page) * c->heads * 2;
-    a.chunk = ctas >= 2ull * s.num_sms ? c->page : 8u;
+    // A prompt's pages hold up to `page` new rows each: 64 rows per CTA and at least a page (4096 tokens, 8 heads of 64, pages of
+    // 16: 9 us, 21 us with 16 rows). Few rows are mostly one per page: eight rows per CTA spread them over the GPU, 16 in
+    // between (1024 rows 4.9 us, 6.2 us with eight).
+    const uint32_t many = c->page > 64 ? c->page : 64;
+    const uint64_t ctas = (uint64_t)((T + many - 1) / many) * c->heads * 2;
+    a.chunk = ctas >= 2ull * s.num_sms ? many : ctas * 4 >= 2ull * s.num_sms ? 16u : 8u;
     const uint32_t gx = (T + a.chunk - 1) / a.chunk;
     if (c->heads * 2ull > 65535) {
         sh::set_error(-1, "[sh_cuda_kv8_append] heads %u > 32767", c->heads);
