@@ -5,14 +5,16 @@
 //
 // Bound by the weights' bytes (half a byte per element, read once), and close behind by the instructions that turn codes
 // into operands, so there are two forms of the inner product, both exact but for fp32 sums:
-//   fp16 (5 to 32 rows)  code - zero is a small integer, exact in fp16: the 16-row operand of the matrix instruction (16
-//        columns of W x 16 k), up to 8 rows of X its columns. 9 instructions turn a word into 8 operands (fp16 patterns
-//        1024 + c and 1024 + 16 c, then one subtraction or FMA).
-//   int8 (1 to 4 rows)   every finite fp16 value is an integer times 2^-24 below 2^41, i.e. six signed base-256 digits. The
-//        codes are int8 operands as they are (3 instructions per 8), the digits of a row of X are six of the instruction's
-//        columns, which single rows would leave empty, and the int32 sums of a group are exact. The zero point
-//        enters as -zero sum(digits). A 16 x 128 step takes 4 matrix instructions and 24 others, not 8 and 72.
-//        Infinities and NaN have no digits; outputs of such a row get those terms one by one.
+//   fp16   code - zero is a small integer, exact in fp16: the 16-row operand of the matrix instruction (16 columns of W x
+//          16 k), up to 8 rows of X its columns. 9 instructions turn a word into 8 operands (fp16 patterns 1024 + c and
+//          1024 + 16 c, then one subtraction or FMA).
+//   int8   for a single row and many columns: every finite fp16 value is an integer times 2^-24 below 2^41, i.e. six signed
+//          base-256 digits. The codes are int8 operands as they are (3 instructions per 8), the digits of X are six of the
+//          instruction's eight columns, of which a single row would leave seven empty, and the int32 sums of a group are
+//          exact. The zero point enters as -zero sum(digits). A 16 x 128 step takes 4 matrix instructions and 24 others, not
+//          8 and 72, but the digits take longer to lay out, so that it pays from about three tiles per SM on
+//          (49152 x 4096: 23.3 us, 30.3 us in fp16; 4096 x 4096: 5.6 us, 4.8 us in fp16).
+//          Infinities and NaN have no digits; outputs of such a row get those terms one by one.
 //
 // One CTA per SM: X is laid out in shared memory once, then groups of 8 warps walk tiles of 16 columns of W, each warp an
 // eighth of K. A warp has its own ring of stages, filled by TMA boxes of 16 columns x 128 bytes with 128-byte swizzle (one
@@ -93,6 +95,7 @@ __device__ __forceinline__ uint32_t tile_row(uint32_t g) { return (g >> 1) | (g 
 
 constexpr uint32_t kGroupWarps = 8, kGroupThreads = 256, kStage = 16 * kUnit / 2;
 constexpr int kDigits = 6;
+constexpr uint32_t kCols = 8, kRows = 16;      // columns of the matrix instruction: rows of X or digits; columns of W per tile
 
 // x 2^24 as six signed base-256 digits: bytes of value + 0x808080808080, each less 128
 __device__ __forceinline__ void digits_of(uint32_t h, uint32_t &lo, uint32_t &hi) {
@@ -118,30 +121,30 @@ __device__ __forceinline__ float small_to_float(int v) { return __int_as_float(v
 struct W4Layout {     // offsets into shared memory
     uint32_t red, part, zero, flag, bars, sc, sc_bytes, xs, x, bytes;
 };
-// cols: columns of the matrix instructions; xcols: those that X fills; steps: of one CTA; gu: quantisation groups per step;
+// steps: of one CTA; gu: quantisation groups per step;
 // groups: of the scales kept; iters: tiles of one group of warps whose sums are kept
-__host__ __device__ inline W4Layout w4_layout(uint32_t ng, uint32_t d, uint32_t cols, uint32_t xcols, uint32_t gu, bool digits,
+__host__ __device__ inline W4Layout w4_layout(uint32_t ng, uint32_t d, uint32_t gu, bool digits,
                                               bool zeros, uint32_t steps, uint32_t m, uint32_t groups, uint32_t iters) {
     W4Layout l;
     uint32_t at = ng * kGroupWarps * d * kStage;
-    l.red = at, at += 2 * ng * kGroupWarps * cols * 16 * 4;
+    l.red = at, at += 2 * ng * kGroupWarps * kCols * 16 * 4;
     l.part = at, at += ng * iters * 16 * m * 4;
     l.zero = at, at += 64;
-    l.flag = at, at += 128;
+    l.flag = at, at += 16;
     l.bars = at, at += ng * (kGroupWarps * d + 2) * 8 + 16;            // and the abort flag
     l.sc_bytes = 16 * groups * (zeros ? 3 : 2);
     l.sc = at, at += 2 * ng * l.sc_bytes;
-    l.xs = at, at += digits ? steps * gu * cols * 4 : 0;
-    l.x = at, at += steps * (digits ? 4 * xcols * 64 : 8 * m * 64);
+    l.xs = at, at += digits ? steps * gu * kCols * 4 : 0;
+    l.x = at, at += steps * (digits ? 4 * kDigits * 64 : 8 * m * 64);
     l.bytes = at + 1024;       // the ring starts on a multiple of 1024
     return l;
 }
 
-// NT: groups of 8 columns of the matrix instruction; INT: digits; NG: groups of 8 warps; D: stages; Z: zero points given
-template <int G, int NT, bool INT, int NG, int D, bool Z>
+// INT: digits (M == 1); NG: groups of 8 warps; D: stages; Z: zero points given
+template <int G, bool INT, int NG, int D, bool Z>
 __global__ void __launch_bounds__(NG * kGroupThreads, 1)
     k_gemv_w4(const __grid_constant__ CUtensorMap mw, W4Args a, uint32_t splits, uint32_t tiles, uint32_t iters) {
-    constexpr uint32_t kThreads = NG * kGroupThreads, kCols = 8 * NT, kRows = 16;
+    constexpr uint32_t kThreads = NG * kGroupThreads;
     constexpr int GU = kUnit / G;                                  // quantisation groups per step
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -153,7 +156,7 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
     const uint32_t u0 = border(part), nu = border(part + 1) - u0;                    // steps of this warp per tile
     const uint32_t x0 = border(blockIdx.y * kGroupWarps), x1 = border((blockIdx.y + 1) * kGroupWarps);   // of this CTA
     const uint32_t xcols = INT ? kDigits * a.M : a.M;
-    const W4Layout L = w4_layout(NG, D, kCols, xcols, GU, INT, Z, (units + splits - 1) / splits + 1, a.M, a.staged ? groups : 0,
+    const W4Layout L = w4_layout(NG, D, GU, INT, Z, (units + splits - 1) / splits + 1, a.M, a.staged ? groups : 0,
                                  iters);
     // tiles of this group: the first ones of all SMs before any SM's second ones
     const uint32_t tile0 = grp * gridDim.x + blockIdx.x, tile_step = NG * gridDim.x;
@@ -207,20 +210,22 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
     // ---- X in the order of the operands ------------------------------------------------------------------------------
     uint4 *s_x = reinterpret_cast<uint4 *>(smem + L.x);
     int *s_xs = reinterpret_cast<int *>(smem + L.xs);
-    int *s_flag = reinterpret_cast<int *>(smem + L.flag);      // rows with infinities or NaN
-    if (t < 32) s_flag[t] = 0;
+    int *s_flag = reinterpret_cast<int *>(smem + L.flag);      // INT: the row has infinities or NaN
+    if (t == 0) *s_flag = 0;
     if (t < 16) reinterpret_cast<uint32_t *>(smem + L.zero)[t] = 0;
     if (INT)
         for (uint32_t i = t; i < (x1 - x0) * GU * kCols; i += kThreads) s_xs[i] = 0;
     __syncthreads();
-    for (uint32_t m = 0; m < a.M; ++m)
-        for (uint32_t i = t; i < (x1 - x0) * 32; i += kThreads) {
-            // 8 neighbouring k: word ii of column cc in half u of the CTA's steps
-            const uint32_t u = i >> 4, j = i & 15, at = x0 * kUnit + i * 8;
-            const uint32_t cc = G == 128 ? j >> 2 : G == 64 ? (j >> 1) & 3 : j & 3;
-            const uint32_t ii = G == 128 ? j & 3 : G == 64 ? (j >> 3) * 2 + (j & 1) : j >> 2;
-            uint32_t x[4] = {0, 0, 0, 0};
-            if (at < a.K) {
+    const uint32_t per_row = (x1 - x0) * 32;      // pieces of 8 neighbouring k in this CTA's steps
+    constexpr uint32_t kBatch = INT ? 1 : 4;      // pieces per thread in flight
+    for (uint32_t p0 = t; p0 < per_row * a.M; p0 += kBatch * kThreads) {
+        uint32_t xs[kBatch][4];
+#pragma unroll
+        for (uint32_t q = 0; q < kBatch; ++q) {
+            const uint32_t p = p0 + q * kThreads, m = p / per_row, at = x0 * kUnit + (p - m * per_row) * 8;
+            uint32_t (&x)[4] = xs[q];
+            x[0] = x[1] = x[2] = x[3] = 0;
+            if (p < per_row * a.M && at < a.K) {
                 const __half *xp = a.x + (size_t)m * a.ldx + at;
                 if (a.vec) {
                     const uint4 v = __ldg(reinterpret_cast<const uint4 *>(xp));
@@ -230,6 +235,16 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
                     for (int e = 0; e < 8; ++e) x[e >> 1] |= (uint32_t)__half_as_ushort(xp[e]) << (16 * (e & 1));
                 }
             }
+        }
+#pragma unroll
+        for (uint32_t q = 0; q < kBatch; ++q) {
+            const uint32_t p = p0 + q * kThreads, m = p / per_row, i = p - m * per_row;
+            if (p >= per_row * a.M) continue;
+            // word ii of column cc in half u of the CTA's steps
+            const uint32_t u = i >> 4, j = i & 15;
+            const uint32_t cc = G == 128 ? j >> 2 : G == 64 ? (j >> 1) & 3 : j & 3;
+            const uint32_t ii = G == 128 ? j & 3 : G == 64 ? (j >> 3) * 2 + (j & 1) : j >> 2;
+            const uint32_t (&x)[4] = xs[q];
             if (!INT) {
                 // pairs (0, 4), (1, 5), (2, 6), (3, 7) as w4_word's; [half][word][row][c]
                 s_x[((u * 4 + ii) * a.M + m) * 4 + cc] =
@@ -241,7 +256,7 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     special |= (x[e] & 0x7C00u) == 0x7C00u || (x[e] & 0x7C000000u) == 0x7C000000u;
-                if (special) s_flag[m] = 1;
+                if (special) *s_flag = 1;
                 uint32_t d[2][kDigits];
 #pragma unroll
                 for (int odd = 0; odd < 2; ++odd) {
@@ -255,34 +270,30 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
                     d[odd][2] = __byte_perm(p2, p3, 0x5410), d[odd][3] = __byte_perm(p2, p3, 0x7632);
                     d[odd][4] = __byte_perm(p4, p5, 0x5410), d[odd][5] = __byte_perm(p4, p5, 0x7632);
                 }
-                const uint32_t q = G == 128 ? 0 : G == 64 ? ii >> 1 : ii;
+                const uint32_t grp_q = G == 128 ? 0 : G == 64 ? ii >> 1 : ii;
 #pragma unroll
                 for (int k = 0; k < kDigits; ++k) {
-                    const uint32_t col = m * kDigits + k;
-                    uint2 *dst = reinterpret_cast<uint2 *>(s_x + ((u * 2 + (ii >> 1)) * xcols + col) * 4 + cc) + (ii & 1);
+                    uint2 *dst = reinterpret_cast<uint2 *>(s_x + ((u * 2 + (ii >> 1)) * kDigits + k) * 4 + cc) + (ii & 1);
                     *dst = make_uint2(d[0][k], d[1][k]);
                     const int sum = __dp4a((int)d[0][k], 0x01010101, __dp4a((int)d[1][k], 0x01010101, 0));
-                    if (sum) atomicAdd(s_xs + (u * (GU / 2) + q) * kCols + col, sum);
+                    if (sum) atomicAdd(s_xs + (u * (GU / 2) + grp_q) * kCols + k, sum);
                 }
             }
         }
+    }
     __syncthreads();
 
-    // this lane's operand column of X in each column group; the zero line where X has none
-    uint32_t bx[NT], bstep[NT];
+    // this lane's operand column of X; the zero line where X has none
     constexpr uint32_t kPieces = INT ? 4 : 8;        // 16-byte pieces of a step per lane
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const bool in = nt * 8 + g < xcols;
-        bx[nt] = smem_u32(smem) + (in ? L.x + (((u0 - x0) * kPieces * xcols + nt * 8 + g) * 4 + c) * 16 : L.zero);
-        bstep[nt] = in ? xcols * 64 : 0;
-    }
+    const bool has_col = g < xcols;
+    const uint32_t bx = smem_u32(smem) + (has_col ? L.x + (((u0 - x0) * kPieces * xcols + g) * 4 + c) * 16 : L.zero);
+    const uint32_t bstep = has_col ? xcols * 64 : 0;
     float *s_red0 = reinterpret_cast<float *>(smem + L.red) + grp * (2 * kGroupWarps * kCols * kRows);
-    // one row of X: the quad's columns are its digits, and only their sums go through shared memory
+    // INT: the quad's columns are digits of one value, and only their sum goes through shared memory
     const float weight = __int_as_float((127 - 24 + 16 * (int)min(c, 2u)) << 23);
     float *s_part = reinterpret_cast<float *>(smem + L.part) + grp * iters * kRows * a.M;
     auto group_sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(grp + 1), "n"(kGroupThreads) : "memory"); };
-    auto finish = [&](float v, uint32_t m, uint32_t n, bool special) {
+    auto finish = [&](float v, uint32_t m, uint32_t n, bool special, float bias, float res) {
         if (INT && special)
             for (uint32_t k = 0; k < a.K; ++k) {
                 const float x = __half2float(a.x[(size_t)m * a.ldx + k]);
@@ -292,22 +303,28 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
                     v = fmaf(((float)code - (float)zero) * __half2float(a.scales[(size_t)n * groups + k / G]), x, v);
                 }
             }
-        if (a.bias) v += __half2float(a.bias[n]);
-        if (a.res) v += __half2float(a.res[(size_t)m * a.ldr + n]);
+        v += bias;
+        v += res;
         a.z[(size_t)m * a.ldz + n] = __float2half_rn(v);
     };
+
+    auto bias_of = [&](uint32_t n) { return a.bias ? __half2float(a.bias[n]) : 0.f; };
+    auto res_of = [&](uint32_t m, uint32_t n) { return a.res ? __half2float(a.res[(size_t)m * a.ldr + n]) : 0.f; };
+    // The output of a thread in each tile: at most one. A single row's sixteen go to the warps in turn.
+    const uint32_t om = INT ? 0 : gt / kRows, orow = gt % kRows;
 
     const uint32_t swz = tile_row(g), w_at = smem_u32(ring) + swz * 128;
     uint32_t slot = 0, phase = 0, iter = 0;
     for (uint32_t tile = tile0; tile < tiles; tile += tile_step, ++iter) {
         const uint32_t turn = iter & 1;
-        float acc[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
-        uint32_t bat[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) bat[nt] = bx[nt];
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t bat = bx;
         const int *xs = s_xs + (u0 - x0) * GU * kCols + 2 * c;
+        // what the output adds is on its way while the products are taken
+        const uint32_t on = tile * kRows + orow;
+        const bool mine = INT ? gw == (iter & 7) && lane < kRows : om < a.M;
+        const bool writes = mine && on < a.N && splits == 1;
+        const float bias = writes ? bias_of(on) : 0.f, res = writes ? res_of(om, on) : 0.f;
         const bool in_smem = staged(tile);
         const uint32_t sat = sc0 + turn * L.sc_bytes + 2 * (swz * groups + u0 * GU);
         const uint32_t zat = sc0 + turn * L.sc_bytes + 2 * kRows * groups + swz * groups + u0 * GU;
@@ -374,53 +391,41 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
                         }
                     }
                 }
-                int gi[NT][4];        // sums of a quantisation group: INT
-                float gf[NT][4];      // or fp16
-                uint32_t b[NT][4];
+                int gi[4];        // sums of a quantisation group: INT
+                float gf[4];      // or fp16
+                uint32_t b[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int q = half * (GU / 2) + i / kPer;
                     const int z0 = (int)z[0][q], z1 = (int)z[1][q];
                     if (i % kPer == 0) {
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            if (INT) {
-                                const int2 y = *reinterpret_cast<const int2 *>(xs + q * kCols + nt * 8);
-                                gi[nt][0] = -z0 * y.x, gi[nt][1] = -z0 * y.y, gi[nt][2] = -z1 * y.x, gi[nt][3] = -z1 * y.y;
-                            } else {
-                                gf[nt][0] = gf[nt][1] = gf[nt][2] = gf[nt][3] = 0.f;
-                            }
+                        if (INT) {
+                            const int2 y = *reinterpret_cast<const int2 *>(xs + q * kCols);
+                            gi[0] = -z0 * y.x, gi[1] = -z0 * y.y, gi[2] = -z1 * y.x, gi[3] = -z1 * y.y;
+                        } else {
+                            gf[0] = gf[1] = gf[2] = gf[3] = 0.f;
                         }
                     }
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        if (!INT || i % 2 == 0) {
-                            load_shared<4>(b[nt], bat[nt]);
-                            bat[nt] += bstep[nt];
-                        }
+                    if (!INT || i % 2 == 0) {
+                        load_shared<4>(b, bat);
+                        bat += bstep;
+                    }
                     if (INT) {
                         const uint32_t a0 = w[0][i] & 0x0F0F0F0Fu, a2 = (w[0][i] >> 4) & 0x0F0F0F0Fu;
                         const uint32_t a1 = w[1][i] & 0x0F0F0F0Fu, a3 = (w[1][i] >> 4) & 0x0F0F0F0Fu;
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-                            w4_imma(gi[nt], a0, a1, a2, a3, b[nt][i % 2 * 2], b[nt][i % 2 * 2 + 1]);
+                        w4_imma(gi, a0, a1, a2, a3, b[i % 2 * 2], b[i % 2 * 2 + 1]);
                     } else {
                         uint32_t h0[4], h1[4];
                         const uint32_t y0 = (uint32_t)z0 * 0x00010001u, y1 = (uint32_t)z1 * 0x00010001u;
                         w4_word(w[0][i], 0x64006400u | y0, 0xD400D400u | y0 << 4, h0);
                         w4_word(w[1][i], 0x64006400u | y1, 0xD400D400u | y1 << 4, h1);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            w4_mma(gf[nt], h0[0], h1[0], h0[1], h1[1], b[nt][0], b[nt][1]);
-                            w4_mma(gf[nt], h0[2], h1[2], h0[3], h1[3], b[nt][2], b[nt][3]);
-                        }
+                        w4_mma(gf, h0[0], h1[0], h0[1], h1[1], b[0], b[1]);
+                        w4_mma(gf, h0[2], h1[2], h0[3], h1[3], b[2], b[3]);
                     }
                     if (i % kPer == kPer - 1) {
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                acc[nt][e] = fmaf(INT ? small_to_float(gi[nt][e]) : gf[nt][e], s[e >> 1][q], acc[nt][e]);
+                        for (int e = 0; e < 4; ++e)
+                            acc[e] = fmaf(INT ? small_to_float(gi[e]) : gf[e], s[e >> 1][q], acc[e]);
                     }
                 }
             }
@@ -431,52 +436,30 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
         // ---- partial sums of the K parts, in their order. A buffer is written again two tiles later, behind the barrier
         // of the tile between, which no warp passes before all have read it; the warps take turns at reading. ---------------
         float *s_red = s_red0 + turn * (kGroupWarps * kCols * kRows);
-        if (INT && NT == 1) {
+        if (INT) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                float v = c < 3 ? fmaf(acc[0][2 * e + 1], 256.f, acc[0][2 * e]) * weight : 0.f;
+                float v = c < 3 ? fmaf(acc[2 * e + 1], 256.f, acc[2 * e]) * weight : 0.f;
                 v += __shfl_xor_sync(0xffffffffu, v, 1);
                 v += __shfl_xor_sync(0xffffffffu, v, 2);
                 if (c == 0) s_red[gw * kRows + swz + 8 * e] = v;
             }
         } else {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    s_red[(gw * kCols + nt * 8 + 2 * c + (e & 1)) * kRows + swz + 8 * (e >> 1)] = acc[nt][e];
+            for (int e = 0; e < 4; ++e) s_red[(gw * kCols + 2 * c + (e & 1)) * kRows + swz + 8 * (e >> 1)] = acc[e];
         }
         fence_proxy_async_smem();      // this tile's scales have been read: their buffer is copied into again
         group_sync();
         fetch_scales(tile + 2 * tile_step, turn);
-        if (INT && NT == 1) {
-            if (gw == (iter & 7) && lane < kRows) {      // the warps take turns
-                const uint32_t n = tile * kRows + lane;
-                float v = 0.f;
+        float v = 0.f;
+        if (mine) {
 #pragma unroll
-                for (uint32_t w = 0; w < kGroupWarps; ++w) v += s_red[w * kRows + lane];
-                if (splits > 1) s_part[iter * kRows + lane] = v;
-                else if (n < a.N) finish(v, 0, n, s_flag[0]);
-            }
-        } else {
-            // INT: eight lanes per output, lane k sums digit k over the warps
-            constexpr uint32_t kLanes = INT ? 8 : 1;
-            for (uint32_t i = gt; i < kLanes * kRows * a.M; i += kGroupThreads) {
-                const uint32_t k = i % kLanes, m = i / (kLanes * kRows), r = i / kLanes % kRows, n = tile * kRows + r;
-                float v = 0.f;
-                if (!INT || k < kDigits) {
-#pragma unroll
-                    for (uint32_t w = 0; w < kGroupWarps; ++w) v += s_red[(w * kCols + (INT ? m * kDigits + k : m)) * kRows + r];
-                }
-                if (INT) {
-                    v *= __int_as_float((127 - 24 + 8 * k) << 23);
-#pragma unroll
-                    for (int d = 1; d < 8; d <<= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-                    if (k) continue;
-                }
-                if (splits > 1) s_part[(iter * a.M + m) * kRows + r] = v;
-                else if (n < a.N) finish(v, m, n, s_flag[m]);
-            }
+            for (uint32_t w = 0; w < kGroupWarps; ++w) v += s_red[INT ? w * kRows + orow : (w * kCols + om) * kRows + orow];
+        }
+        if (splits > 1) {
+            if (mine) s_part[(iter * a.M + om) * kRows + orow] = v;
+        } else if (writes) {
+            finish(v, om, on, *s_flag, bias, res);
         }
     }
     if (*abort)      // a copy did not arrive in time: give those in flight as long again
@@ -488,7 +471,7 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
             for (uint32_t i = blockIdx.y * kGroupThreads + gt; i < kRows * a.M; i += splits * kGroupThreads) {
                 const uint32_t m = i / kRows, n = tile * kRows + i % kRows;
                 if (n >= a.N) continue;
-                const uint32_t at = smem_u32(s_part + iter * kRows * a.M + i), fat = smem_u32(s_flag + m);
+                const uint32_t at = smem_u32(s_part + iter * kRows * a.M + i), fat = smem_u32(s_flag);
                 float v = 0.f;
                 int special = 0;
                 for (uint32_t k = 0; k < splits; ++k) {
@@ -499,7 +482,7 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
                     v += y;
                     special |= f;
                 }
-                finish(v, m, n, special != 0);
+                finish(v, m, n, special != 0, bias_of(n), res_of(m, n));
             }
         cluster_sync_all();      // the other CTAs have read this one's sums
     }
@@ -520,10 +503,9 @@ bool w4_map(CUtensorMap *m, uint64_t codes, uint32_t N, uint32_t K, uint32_t ldw
 
 constexpr size_t kSmemMax = 227 * 1024, kMaxScales = 64 * 1024;
 
-template <int G, int NT, bool INT, int NG, int D>
+template <int G, bool INT, int NG, int D>
 cudaError_t w4_try(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bool &fits) {
     const uint32_t tiles = (a.N + 15) / 16, units = (a.K + kUnit - 1) / kUnit;
-    const uint32_t xcols = INT ? kDigits * a.M : a.M;
     uint32_t s = 1, room, iters;
     size_t smem;
     // K parts over a cluster while the columns alone leave SMs idle and every warp keeps a step, or until X fits
@@ -532,13 +514,13 @@ cudaError_t w4_try(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bo
         room = (uint32_t)sms / s;
         const uint32_t ctas = tiles < room ? tiles : room;
         iters = s > 1 ? (tiles + ctas * NG - 1) / (ctas * NG) : 0;      // sums kept for the cluster
-        smem = w4_layout(NG, D, 8 * NT, xcols, kUnit / G, INT, a.zeros != nullptr, (units + s - 1) / s + 1, a.M,
+        smem = w4_layout(NG, D, kUnit / G, INT, a.zeros != nullptr, (units + s - 1) / s + 1, a.M,
                          a.staged ? a.K / G : 0, iters).bytes;
         if (s == 8 || !((tiles * s * 2 <= (uint32_t)sms && units >= kGroupWarps * s * 2) || smem > kSmemMax)) break;
     }
     fits = smem <= kSmemMax;
     if (!fits) return cudaSuccess;
-    auto kernel = a.zeros ? k_gemv_w4<G, NT, INT, NG, D, true> : k_gemv_w4<G, NT, INT, NG, D, false>;
+    auto kernel = a.zeros ? k_gemv_w4<G, INT, NG, D, true> : k_gemv_w4<G, INT, NG, D, false>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
@@ -556,22 +538,19 @@ cudaError_t w4_try(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bo
     return cudaLaunchKernelEx(&cfg, kernel, mw, a, s, tiles, iters);
 }
 
-// Rows of X go in pieces of at most 8, and fewer when they do not fit beside each other. A second piece finds the weights
-// in L2 unless they are larger than that. (16 and 32 rows in one pass, with two or four column groups per instruction
-// stream and X shared by a cluster: 14336 x 4096 29 us and 60 us, against 2 and 4 passes of 16 us.)
+// Rows of X go in pieces of at most 8, and fewer when they do not fit beside each other. A second piece finds the weights in
+// L2 unless they are larger than that. (16 rows in one pass, with two column groups per instruction stream and X shared by a
+// cluster: 14336 x 4096 30 us, against 2 passes of 12.9 us.)
 template <int G>
 cudaError_t w4_run(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bool &fits) {
     cudaError_t e = cudaSuccess;
     fits = false;
-    if (a.M == 1) {
-        e = w4_try<G, 1, true, 3, 2>(a, mw, sms, st, fits);
-        // long K: one group of warps, whose scales and fp16 row of X take least shared memory
-        if (!fits && e == cudaSuccess) e = w4_try<G, 1, false, 1, 3>(a, mw, sms, st, fits);
-        return e;
-    }
-    if (a.M == 2) e = w4_try<G, 2, true, 3, 2>(a, mw, sms, st, fits);
-    else if (a.M <= 8) e = w4_try<G, 1, false, 3, 2>(a, mw, sms, st, fits);
-    if (fits || e != cudaSuccess) return e;
+    const uint32_t tiles = (a.N + 15) / 16;
+    if (a.M == 1 && tiles >= 3u * sms) e = w4_try<G, true, 3, 2>(a, mw, sms, st, fits);
+    if (!fits && e == cudaSuccess && a.M <= 8) e = w4_try<G, false, 3, 2>(a, mw, sms, st, fits);
+    // long K: one group of warps, whose scales take less shared memory
+    if (!fits && e == cudaSuccess && a.M == 1) e = w4_try<G, false, 1, 3>(a, mw, sms, st, fits);
+    if (fits || e != cudaSuccess || a.M == 1) return e;
     const uint32_t first = a.M > 8 ? 8 : a.M / 2, M = a.M;
     a.M = first;
     e = w4_run<G>(a, mw, sms, st, fits);
