@@ -6,7 +6,7 @@
 // Bound by the weights' bytes (half a byte per element, read once), and close behind by the instructions that turn codes
 // into operands, so there are two forms of the inner product, both exact but for fp32 sums:
 //   fp16   code - zero is a small integer, exact in fp16: the 16-row operand of the matrix instruction (16 columns of W x
-//          16 k), up to 8 rows of X its columns. 9 instructions turn a word into 8 operands (fp16 patterns 1024 + c and
+//          16 k), 8 rows of X its columns, twice for up to 16 rows. 9 instructions turn a word into 8 operands (fp16 patterns 1024 + c and
 //          1024 + 16 c, then one subtraction or FMA).
 //   int8   for a single row and many columns: every finite fp16 value is an integer times 2^-24 below 2^41, i.e. six signed
 //          base-256 digits. The codes are int8 operands as they are (3 instructions per 8), the digits of X are six of the
@@ -95,7 +95,7 @@ __device__ __forceinline__ uint32_t tile_row(uint32_t g) { return (g >> 1) | (g 
 
 constexpr uint32_t kGroupWarps = 8, kGroupThreads = 256, kStage = 16 * kUnit / 2;
 constexpr int kDigits = 6;
-constexpr uint32_t kCols = 8, kRows = 16;      // columns of the matrix instruction: rows of X or digits; columns of W per tile
+constexpr uint32_t kRows = 16;      // columns of W per tile
 
 // x 2^24 as six signed base-256 digits: bytes of value + 0x808080808080, each less 128
 __device__ __forceinline__ void digits_of(uint32_t h, uint32_t &lo, uint32_t &hi) {
@@ -121,30 +121,30 @@ __device__ __forceinline__ float small_to_float(int v) { return __int_as_float(v
 struct W4Layout {     // offsets into shared memory
     uint32_t red, part, zero, flag, bars, sc, sc_bytes, xs, x, bytes;
 };
-// steps: of one CTA; gu: quantisation groups per step;
+// nt: groups of 8 columns of the matrix instruction; steps: of one CTA; gu: quantisation groups per step;
 // groups: of the scales kept; iters: tiles of one group of warps whose sums are kept
-__host__ __device__ inline W4Layout w4_layout(uint32_t ng, uint32_t d, uint32_t gu, bool digits,
+__host__ __device__ inline W4Layout w4_layout(uint32_t ng, uint32_t d, uint32_t nt, uint32_t gu, bool digits,
                                               bool zeros, uint32_t steps, uint32_t m, uint32_t groups, uint32_t iters) {
     W4Layout l;
     uint32_t at = ng * kGroupWarps * d * kStage;
-    l.red = at, at += 2 * ng * kGroupWarps * kCols * 16 * 4;
+    l.red = at, at += (nt == 1 ? 2 : 1) * ng * kGroupWarps * 8 * nt * 16 * 4;
     l.part = at, at += ng * iters * 16 * m * 4;
     l.zero = at, at += 64;
     l.flag = at, at += 16;
     l.bars = at, at += ng * (kGroupWarps * d + 2) * 8 + 16;            // and the abort flag
     l.sc_bytes = 16 * groups * (zeros ? 3 : 2);
     l.sc = at, at += 2 * ng * l.sc_bytes;
-    l.xs = at, at += digits ? steps * gu * kCols * 4 : 0;
+    l.xs = at, at += digits ? steps * gu * 8 * 4 : 0;
     l.x = at, at += steps * (digits ? 4 * kDigits * 64 : 8 * m * 64);
     l.bytes = at + 1024;       // the ring starts on a multiple of 1024
     return l;
 }
 
-// INT: digits (M == 1); NG: groups of 8 warps; D: stages; Z: zero points given
-template <int G, bool INT, int NG, int D, bool Z>
+// INT: digits (M == 1); NT: groups of 8 columns of the matrix instruction; NG: groups of 8 warps; D: stages; Z: zero points given
+template <int G, bool INT, int NT, int NG, int D, bool Z>
 __global__ void __launch_bounds__(NG * kGroupThreads, 1)
     k_gemv_w4(const __grid_constant__ CUtensorMap mw, W4Args a, uint32_t splits, uint32_t tiles, uint32_t iters) {
-    constexpr uint32_t kThreads = NG * kGroupThreads;
+    constexpr uint32_t kThreads = NG * kGroupThreads, kCols = 8 * NT;
     constexpr int GU = kUnit / G;                                  // quantisation groups per step
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
     const uint32_t u0 = border(part), nu = border(part + 1) - u0;                    // steps of this warp per tile
     const uint32_t x0 = border(blockIdx.y * kGroupWarps), x1 = border((blockIdx.y + 1) * kGroupWarps);   // of this CTA
     const uint32_t xcols = INT ? kDigits * a.M : a.M;
-    const W4Layout L = w4_layout(NG, D, GU, INT, Z, (units + splits - 1) / splits + 1, a.M, a.staged ? groups : 0,
+    const W4Layout L = w4_layout(NG, D, NT, GU, INT, Z, (units + splits - 1) / splits + 1, a.M, a.staged ? groups : 0,
                                  iters);
     // tiles of this group: the first ones of all SMs before any SM's second ones
     const uint32_t tile0 = grp * gridDim.x + blockIdx.x, tile_step = NG * gridDim.x;
@@ -285,10 +285,14 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
 
     // this lane's operand column of X; the zero line where X has none
     constexpr uint32_t kPieces = INT ? 4 : 8;        // 16-byte pieces of a step per lane
-    const bool has_col = g < xcols;
-    const uint32_t bx = smem_u32(smem) + (has_col ? L.x + (((u0 - x0) * kPieces * xcols + g) * 4 + c) * 16 : L.zero);
-    const uint32_t bstep = has_col ? xcols * 64 : 0;
-    float *s_red0 = reinterpret_cast<float *>(smem + L.red) + grp * (2 * kGroupWarps * kCols * kRows);
+    uint32_t bx[NT], bstep[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const bool has = nt * 8 + g < xcols;
+        bx[nt] = smem_u32(smem) + (has ? L.x + (((u0 - x0) * kPieces * xcols + nt * 8 + g) * 4 + c) * 16 : L.zero);
+        bstep[nt] = has ? xcols * 64 : 0;
+    }
+    float *s_red0 = reinterpret_cast<float *>(smem + L.red) + grp * ((NT == 1 ? 2 : 1) * kGroupWarps * kCols * kRows);
     // INT: the quad's columns are digits of one value, and only their sum goes through shared memory
     const float weight = __int_as_float((127 - 24 + 16 * (int)min(c, 2u)) << 23);
     float *s_part = reinterpret_cast<float *>(smem + L.part) + grp * iters * kRows * a.M;
@@ -317,8 +321,10 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
     uint32_t slot = 0, phase = 0, iter = 0;
     for (uint32_t tile = tile0; tile < tiles; tile += tile_step, ++iter) {
         const uint32_t turn = iter & 1;
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t bat = bx;
+        float acc[NT][4];
+        uint32_t bat[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f, bat[nt] = bx[nt];
         const int *xs = s_xs + (u0 - x0) * GU * kCols + 2 * c;
         // what the output adds is on its way while the products are taken
         const uint32_t on = tile * kRows + orow;
@@ -392,8 +398,8 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
                     }
                 }
                 int gi[4];        // sums of a quantisation group: INT
-                float gf[4];      // or fp16
-                uint32_t b[4];
+                float gf[NT][4];  // or fp16
+                uint32_t b[NT][4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int q = half * (GU / 2) + i / kPer;
@@ -403,29 +409,37 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
                             const int2 y = *reinterpret_cast<const int2 *>(xs + q * kCols);
                             gi[0] = -z0 * y.x, gi[1] = -z0 * y.y, gi[2] = -z1 * y.x, gi[3] = -z1 * y.y;
                         } else {
-                            gf[0] = gf[1] = gf[2] = gf[3] = 0.f;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) gf[nt][0] = gf[nt][1] = gf[nt][2] = gf[nt][3] = 0.f;
                         }
                     }
-                    if (!INT || i % 2 == 0) {
-                        load_shared<4>(b, bat);
-                        bat += bstep;
-                    }
+                    if (!INT || i % 2 == 0)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            load_shared<4>(b[nt], bat[nt]);
+                            bat[nt] += bstep[nt];
+                        }
                     if (INT) {
                         const uint32_t a0 = w[0][i] & 0x0F0F0F0Fu, a2 = (w[0][i] >> 4) & 0x0F0F0F0Fu;
                         const uint32_t a1 = w[1][i] & 0x0F0F0F0Fu, a3 = (w[1][i] >> 4) & 0x0F0F0F0Fu;
-                        w4_imma(gi, a0, a1, a2, a3, b[i % 2 * 2], b[i % 2 * 2 + 1]);
+                        w4_imma(gi, a0, a1, a2, a3, b[0][i % 2 * 2], b[0][i % 2 * 2 + 1]);
                     } else {
                         uint32_t h0[4], h1[4];
                         const uint32_t y0 = (uint32_t)z0 * 0x00010001u, y1 = (uint32_t)z1 * 0x00010001u;
                         w4_word(w[0][i], 0x64006400u | y0, 0xD400D400u | y0 << 4, h0);
                         w4_word(w[1][i], 0x64006400u | y1, 0xD400D400u | y1 << 4, h1);
-                        w4_mma(gf, h0[0], h1[0], h0[1], h1[1], b[0], b[1]);
-                        w4_mma(gf, h0[2], h1[2], h0[3], h1[3], b[2], b[3]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            w4_mma(gf[nt], h0[0], h1[0], h0[1], h1[1], b[nt][0], b[nt][1]);
+                            w4_mma(gf[nt], h0[2], h1[2], h0[3], h1[3], b[nt][2], b[nt][3]);
+                        }
                     }
                     if (i % kPer == kPer - 1) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            acc[e] = fmaf(INT ? small_to_float(gi[e]) : gf[e], s[e >> 1][q], acc[e]);
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                acc[nt][e] = fmaf(INT ? small_to_float(gi[e]) : gf[nt][e], s[e >> 1][q], acc[nt][e]);
                     }
                 }
             }
@@ -433,20 +447,23 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
             issue();      // into the stage just read
         }
 
-        // ---- partial sums of the K parts, in their order. A buffer is written again two tiles later, behind the barrier
-        // of the tile between, which no warp passes before all have read it; the warps take turns at reading. ---------------
-        float *s_red = s_red0 + turn * (kGroupWarps * kCols * kRows);
+        // ---- partial sums of the K parts, in their order. With two buffers one is written again two tiles later, behind the
+        // barrier of the tile between, which no warp passes before all have read it; one buffer takes a second barrier. -----
+        float *s_red = s_red0 + (NT == 1 ? turn : 0) * (kGroupWarps * kCols * kRows);
         if (INT) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                float v = c < 3 ? fmaf(acc[2 * e + 1], 256.f, acc[2 * e]) * weight : 0.f;
+                float v = c < 3 ? fmaf(acc[0][2 * e + 1], 256.f, acc[0][2 * e]) * weight : 0.f;
                 v += __shfl_xor_sync(0xffffffffu, v, 1);
                 v += __shfl_xor_sync(0xffffffffu, v, 2);
                 if (c == 0) s_red[gw * kRows + swz + 8 * e] = v;
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s_red[(gw * kCols + 2 * c + (e & 1)) * kRows + swz + 8 * (e >> 1)] = acc[e];
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    s_red[(gw * kCols + nt * 8 + 2 * c + (e & 1)) * kRows + swz + 8 * (e >> 1)] = acc[nt][e];
         }
         fence_proxy_async_smem();      // this tile's scales have been read: their buffer is copied into again
         group_sync();
@@ -461,6 +478,7 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
         } else if (writes) {
             finish(v, om, on, *s_flag, bias, res);
         }
+        if (NT > 1) group_sync();
     }
     if (*abort)      // a copy did not arrive in time: give those in flight as long again
         for (int d = 0; d < D; ++d) drain_wait(full + d, phase ^ (d < (int)slot));
@@ -503,7 +521,7 @@ bool w4_map(CUtensorMap *m, uint64_t codes, uint32_t N, uint32_t K, uint32_t ldw
 
 constexpr size_t kSmemMax = 227 * 1024, kMaxScales = 64 * 1024;
 
-template <int G, bool INT, int NG, int D>
+template <int G, bool INT, int NT, int NG, int D>
 cudaError_t w4_try(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bool &fits) {
     const uint32_t tiles = (a.N + 15) / 16, units = (a.K + kUnit - 1) / kUnit;
     uint32_t s = 1, room, iters;
@@ -514,13 +532,13 @@ cudaError_t w4_try(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bo
         room = (uint32_t)sms / s;
         const uint32_t ctas = tiles < room ? tiles : room;
         iters = s > 1 ? (tiles + ctas * NG - 1) / (ctas * NG) : 0;      // sums kept for the cluster
-        smem = w4_layout(NG, D, kUnit / G, INT, a.zeros != nullptr, (units + s - 1) / s + 1, a.M,
+        smem = w4_layout(NG, D, NT, kUnit / G, INT, a.zeros != nullptr, (units + s - 1) / s + 1, a.M,
                          a.staged ? a.K / G : 0, iters).bytes;
         if (s == 8 || !((tiles * s * 2 <= (uint32_t)sms && units >= kGroupWarps * s * 2) || smem > kSmemMax)) break;
     }
     fits = smem <= kSmemMax;
     if (!fits) return cudaSuccess;
-    auto kernel = a.zeros ? k_gemv_w4<G, INT, NG, D, true> : k_gemv_w4<G, INT, NG, D, false>;
+    auto kernel = a.zeros ? k_gemv_w4<G, INT, NT, NG, D, true> : k_gemv_w4<G, INT, NT, NG, D, false>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
@@ -538,20 +556,20 @@ cudaError_t w4_try(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bo
     return cudaLaunchKernelEx(&cfg, kernel, mw, a, s, tiles, iters);
 }
 
-// Rows of X go in pieces of at most 8, and fewer when they do not fit beside each other. A second piece finds the weights in
-// L2 unless they are larger than that. (16 rows in one pass, with two column groups per instruction stream and X shared by a
-// cluster: 14336 x 4096 30 us, against 2 passes of 12.9 us.)
+// Rows of X go in pieces of at most 16, and fewer when they do not fit beside each other. A second piece finds the weights
+// in L2 unless they are larger than that.
 template <int G>
 cudaError_t w4_run(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bool &fits) {
     cudaError_t e = cudaSuccess;
     fits = false;
     const uint32_t tiles = (a.N + 15) / 16;
-    if (a.M == 1 && tiles >= 3u * sms) e = w4_try<G, true, 3, 2>(a, mw, sms, st, fits);
-    if (!fits && e == cudaSuccess && a.M <= 8) e = w4_try<G, false, 3, 2>(a, mw, sms, st, fits);
+    if (a.M == 1 && tiles >= 3u * sms) e = w4_try<G, true, 1, 3, 2>(a, mw, sms, st, fits);
+    if (!fits && e == cudaSuccess && a.M <= 8) e = w4_try<G, false, 1, 3, 2>(a, mw, sms, st, fits);
+    if (e == cudaSuccess && a.M > 8 && a.M <= 16) e = w4_try<G, false, 2, 2, 2>(a, mw, sms, st, fits);
     // long K: one group of warps, whose scales take less shared memory
-    if (!fits && e == cudaSuccess && a.M == 1) e = w4_try<G, false, 1, 3>(a, mw, sms, st, fits);
+    if (!fits && e == cudaSuccess && a.M == 1) e = w4_try<G, false, 1, 1, 3>(a, mw, sms, st, fits);
     if (fits || e != cudaSuccess || a.M == 1) return e;
-    const uint32_t first = a.M > 8 ? 8 : a.M / 2, M = a.M;
+    const uint32_t first = a.M > 16 ? 16 : a.M > 8 ? 8 : a.M / 2, M = a.M;
     a.M = first;
     e = w4_run<G>(a, mw, sms, st, fits);
     if (e != cudaSuccess || !fits) return e;

@@ -526,6 +526,15 @@ def test_w4_columns_and_depths(gpu_lib, group, N):
         _w4_case(gpu_lib, 5, N, k * group, group, False)
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_w4_single_row_of_many_columns(gpu_lib, group, zeros):
+    """Enough columns for the exact integer products: K inside a step, odd numbers of groups, a last tile that is not full."""
+    for k in (1, 3, 8, 17):
+        _w4_case(gpu_lib, 1, 7201, k * group, group, zeros, L.EPI_RESIDUAL)
+    _w4_case(gpu_lib, 1, 7200, 2048, group, zeros, L.EPI_BIAS, ldx=2055, offset=1)
+
+
 @pytest.mark.parametrize("M", [1, 12])
 def test_w4_strides_and_odd_addresses(gpu_lib, M):
     for ldx, ldz, ldw, offset in ((520, 100, 256, 0), (513, 97, 272, 0), (512, 96, 1024, 1)):
@@ -542,7 +551,7 @@ def test_w4_deep(gpu_lib, M, K, group):
 def test_w4_is_deterministic_and_exact_on_whole_numbers(gpu_lib):
     """Small whole numbers: every product and sum is exact, so each term is counted once and in its place."""
     rt, rng = gpu_lib, np.random.default_rng(5)
-    for M, N, K, group in ((1, 700, 4096, 128), (3, 333, 2016, 32), (32, 130, 8192, 64)):
+    for M, N, K, group in ((1, 700, 4096, 128), (1, 7300, 1056, 32), (3, 333, 2016, 32), (13, 130, 4096, 64), (32, 130, 8192, 64)):
         codes = rng.integers(0, 256, (N, K // 2)).astype(np.uint8)
         scales = rng.integers(1, 3, (N, K // group)).astype(np.float16)
         x = rng.integers(-1, 2, (M, K)).astype(np.float16) * (rng.random((M, K)) < 0.05)
@@ -555,10 +564,10 @@ def test_w4_is_deterministic_and_exact_on_whole_numbers(gpu_lib):
         np.testing.assert_array_equal(_np(z).astype(np.float64), want)
 
 
-@pytest.mark.parametrize("M", [2, 3, 6, 12])
-@pytest.mark.parametrize("N,K", [(64, 256), (40, 16384)])
+@pytest.mark.parametrize("M,N,K", [(2, 64, 256), (6, 64, 256), (12, 40, 16384), (2, 40, 16384), (1, 7201, 256), (1, 7201, 1024)])
 def test_w4_special_rows_stay_apart(gpu_lib, M, N, K):
     """Infinity and NaN in one row of X reach that row of Z only, as IEEE sums have them."""
+    at = min(1, M - 1)
     rt = gpu_lib
     x = torch.randn((M, K), device=DEV).half()
     codes = torch.randint(0, 256, (N, K // 2), device=DEV, dtype=torch.uint8)
@@ -570,26 +579,26 @@ def test_w4_special_rows_stay_apart(gpu_lib, M, N, K):
         rt.check()
         return _np(z)
     good = run(x)
-    rest = [i for i in range(M) if i != 1]
+    rest = [i for i in range(M) if i != at]
     W = D.w4_weights(_np(codes), _np(scales), None, 128, K)
     for specials in ({17: np.nan, 200: np.inf}, {K - 1: np.inf}, {5: -np.inf}, {5: np.inf, 9: np.inf}):
         y = x.clone()
         for k, v in specials.items():
-            y[1, k] = v
+            y[at, k] = v
         got = run(y)
         assert np.array_equal(got[rest], good[rest])
         with np.errstate(invalid="ignore"):
             want = sum(W[k] * v for k, v in specials.items())          # inf, -inf, or NaN where a weight is 0
-        assert np.array_equal(np.isnan(got[1]), np.isnan(want))
+        assert np.array_equal(np.isnan(got[at]), np.isnan(want))
         ok = ~np.isnan(want)
-        assert np.array_equal(got[1][ok].astype(np.float64), want[ok])
+        assert np.array_equal(got[at][ok].astype(np.float64), want[ok])
 
 
-@pytest.mark.parametrize("M", [1, 2, 4])
-def test_w4_wide_range_of_x(gpu_lib, M):
+@pytest.mark.parametrize("M,N", [(1, 90), (4, 90), (1, 7201)])
+def test_w4_wide_range_of_x(gpu_lib, M, N):
     """fp16 values from the smallest to the largest in one row: small ones beside weights that cancel or skip the large."""
     rt, rng = gpu_lib, np.random.default_rng(7)
-    N, K, group = 90, 512, 64
+    K, group = 512, 64
     codes = rng.integers(0, 256, (N, K // 2)).astype(np.uint8)
     codes[::2, :64] = 0x88                              # zero weights below the large values
     scales = rng.uniform(0.5, 1.5, (N, K // group)).astype(np.float16) * np.float16(2.0 ** -6)
