@@ -348,7 +348,7 @@ def test_attention_rows_without_keys(gpu_lib):
     assert (got[:38] == 0).all() and (got[40:70] == 0).all()
 
 
-@pytest.mark.parametrize("nq", [1, 3, 40])
+@pytest.mark.parametrize("nq", [1, 3, 40, 90])
 def test_attention_strides_and_odd_addresses(gpu_lib, nq):
     for ldq, ldo, offset in ((4 * 64 + 8, 4 * 64 + 2, 0), (4 * 64 + 3, 4 * 64 + 1, 0), (4 * 64, 4 * 64, 1)):
         _attn_case(gpu_lib, "int8", 4, 2, 64, 32, [50, 140], [nq, nq], ldq=ldq, ldo=ldo, offset=offset, interleaved=True)
@@ -360,13 +360,13 @@ def test_attention_max_q_only_picks_the_kernel(gpu_lib, max_q):
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.125, 3.0])
-@pytest.mark.parametrize("nq", [1, 30])
+@pytest.mark.parametrize("nq", [1, 30, 80])
 def test_attention_scales_of_the_softmax(gpu_lib, scale, nq):
     _attn_case(gpu_lib, "int8", 4, 2, 64, 16, [300, 47], [nq, nq], scale=scale)
 
 
 @pytest.mark.parametrize("fmt", ["int8", "fp8"])
-@pytest.mark.parametrize("nq", [1, 30])
+@pytest.mark.parametrize("nq", [1, 30, 80])
 def test_attention_scales_far_apart(gpu_lib, fmt, nq):
     """Value scales from 2^-40 to 2^3 and zero (with codes of zero, as the append leaves them) in one request: the
     exponent carries them, so no weight leaves fp16's range."""
@@ -386,7 +386,7 @@ def test_attention_scales_far_apart(gpu_lib, fmt, nq):
     _attn_case(gpu_lib, fmt, 4, 2, 64, 16, [200, 60], [nq, nq], mutate=mutate)
 
 
-@pytest.mark.parametrize("nq", [1, 30])
+@pytest.mark.parametrize("nq", [1, 30, 80])
 def test_attention_ignores_what_lies_behind_a_request(gpu_lib, nq):
     """NaN codes in the rows behind the last token and in free pages, NaN scales of free pages, wild table entries behind the
     request's blocks."""
@@ -403,7 +403,7 @@ def test_attention_ignores_what_lies_behind_a_request(gpu_lib, nq):
     _attn_case(gpu_lib, "fp8", 4, 2, 64, 32, [31, 33, 70, 1 + nq, 128], [1, nq, nq, 1 + nq, 1], mutate=mutate)
 
 
-@pytest.mark.parametrize("nq", [1, 30])
+@pytest.mark.parametrize("nq", [1, 30, 80])
 def test_attention_wrong_tables_and_lengths_are_reported(gpu_lib, nq):
     """A table entry outside the cache and a length past the table: the error word, no fault, other requests intact."""
     rt = gpu_lib
@@ -442,7 +442,7 @@ def test_attention_pages_past_4_gib(gpu_lib):
     scales = torch.full((pages, heads), 0.02, device=DEV)
     h = L.Kv8(_p(pool), _p(pool), _p(scales), _p(scales), size, pages, page, heads, dh, L.SH_INT8)
     ws = torch.zeros(L.KV8_WS_BYTES, dtype=torch.uint8, device=DEV)
-    for nq in (1, 40):
+    for nq in (1, 20, 40):
         q = torch.from_numpy(rng.standard_normal((nq, H * dh)).astype(np.float16)).to(DEV)
         outs = []
         for first in (0, pages - 4):
@@ -471,6 +471,41 @@ def test_attention_many_requests_and_one_long(gpu_lib):
     nq = (np.arange(300) % 3 == 0).astype(int)
     lens[151], nq[151] = 5000, 1
     _attn_case(gpu_lib, "int8", 4, 1, 64, 64, lens, nq)
+
+
+@pytest.mark.parametrize("fmt,dh,scale", [("int8", 64, None), ("fp8", 128, -0.2), ("int8", 128, 2.0)])
+def test_attention_chunks_behind_long_prefixes(gpu_lib, fmt, dh, scale):
+    """Chunks whose keys span many CTAs, with tiles of rows that end inside a request, beside many short ones."""
+    lens, nq = np.full(40, 100), np.where(np.arange(40) % 2, 70, 1)
+    lens[7], nq[7] = 9000, 65
+    lens[20], nq[20] = 4001, 130
+    _attn_case(gpu_lib, fmt, 2, 1, dh, 32, lens, nq, scale=scale)
+
+
+@pytest.mark.parametrize("nq", [1, 12, 80])
+def test_attention_infinite_and_nan_queries_stay_in_their_rows(gpu_lib, nq):
+    """A row of Q with an infinity or a NaN gives NaN for its own head and leaves the others' bits as they were."""
+    rt = gpu_lib
+    pool = Pool(8, 2, 32, 64, "int8", 4)
+    q = torch.randn((2 * nq, 256), device=DEV, generator=torch.Generator(DEV).manual_seed(1)).half()
+    start, table, lens = _i32([0, nq, 2 * nq]), _i32([[0, 1, 2, 3], [4, 5, 6, 7]]), _i32([100, 128])
+    ws = torch.zeros(L.KV8_WS_BYTES, dtype=torch.uint8, device=DEV)
+
+    def run(x):
+        o = torch.zeros_like(x)
+        assert rt.lib.sh_cuda_attention_kv8(_p(x), _p(o), pool.handle, _p(table), 4, _p(lens), _p(start), 2, 2 * nq, nq, 4, 256, 256,
+                                            0.125, _p(ws), ws.numel()) == 0
+        rt.check()
+        return _np(o).view(np.uint16).reshape(2 * nq, 4, 64), _np(o).reshape(2 * nq, 4, 64)
+    good, _ = run(q)
+    for v in (float("inf"), float("nan")):
+        x = q.clone()
+        x[nq, 64 + 9] = v
+        bits, got = run(x)
+        assert np.isnan(got[nq, 1]).all()
+        rest = np.ones(good.shape[:2], bool)
+        rest[nq, 1] = False
+        assert np.array_equal(bits[rest], good[rest])
 
 
 # ---- 4-bit weights -------------------------------------------------------------------------------------------------------
