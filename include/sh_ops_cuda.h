@@ -153,7 +153,8 @@ typedef struct sh_cuda_kv8_t {
  * for row i < t_cap slots[i] = page * (tokens per page) + offset and pos[i] = the token's position in its request (the
  * row of a RoPE table), or slot -1 for the rows of put-off requests, and slot -1, pos 0 for rows past the last token;
  * pool_out = {head, count, number of requests put off, ..}. lens_out may be lens and pool_out may be pool (a running
- * pool); with other addresses a call can be repeated. Words 3..6 of pool_out are left alone, word 7 belongs to the
+ * pool); with other addresses a call can be repeated. lens[r] + add[r] and the sum of all add > 0 stay below 2^31; rows
+ * from t_cap on get table entries but no slot. R == 0 writes nothing. Words 3..6 of pool_out are left alone, word 7 belongs to the
  * library: zero before the first call. Returns 0 or -1 (reason printed). */
 int sh_cuda_kv_tables(uint64_t lens, uint64_t add, uint32_t R, uint32_t page, uint64_t table, uint32_t ld_table,
                       uint64_t ring, uint32_t pages, uint64_t pool, uint64_t pool_out, uint64_t lens_out,
@@ -190,8 +191,8 @@ int sh_cuda_attention_kv8(uint64_t q, uint64_t o, const sh_cuda_kv8_t *cache, ui
  * >= K / 2; 16-byte aligned) holds the codes of column n of W, k = 2 i in the low and k = 2 i + 1 in the high half of
  * byte i, and W[k, n] = scales[n, k / group] * (code - zeros[n, k / group]): fp16 scales and uint8 zero points (0..15)
  * of K / group columns, zeros == 0 meaning 8 everywhere. group 32, 64 or 128, K % group == 0, K <= 262144. X, Z fp16 with
- * leading dims ldx, ldz; fp32 accumulation in a fixed order. flags: SH_EPI_BIAS and SH_EPI_RESIDUAL as in sh_cuda_gemm (Z may be
- * the residual, not X). Returns 0 or -1 (reason printed). */
+ * leading dims ldx, ldz; fp32 accumulation in a fixed order. flags: SH_EPI_BIAS and SH_EPI_RESIDUAL as in sh_cuda_gemm
+ * (Z may be the residual, not X). Returns 0 or -1 (reason printed). */
 int sh_cuda_gemv_w4(uint64_t x, uint64_t codes, uint64_t scales, uint64_t zeros, uint64_t z, uint32_t M, uint32_t N,
                     uint32_t K, uint32_t ldx, uint32_t ldw, uint32_t ldz, uint32_t group, uint64_t bias,
                     uint64_t residual, uint32_t ldr, uint32_t flags);

@@ -190,7 +190,8 @@ template <int DH, int NT, int NW, bool FP8>
 __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
     k_attn_kv8_rows(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, KvArgs a) {
     using SM = RowsSmem<DH, NT, NW>;
-    constexpr uint32_t RT = 8 * NT, kThreads = NW * 32, kStep = SM::kTokens, kKeys = kStep * NW;      // rows of a tile, keys per unit
+    constexpr uint32_t RT = 8 * NT, kThreads = NW * 32;                     // rows of a tile
+    constexpr uint32_t kStep = SM::kTokens, kKeys = kStep * NW;             // keys of a warp's step, of a unit
     constexpr int KC = DH / 64;                     // 16-byte pieces of a K row per lane
     constexpr int VB = DH / 8;                      // V columns per lane
     constexpr int VW = VB / 4;                      // as words
@@ -585,7 +586,7 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
                     for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
                     for (uint32_t i = lane; i < parts; i += 32) {
                         const float mi = __ldcg(part(i) + RT * DH + n);
-                        if (mi != -INFINITY) ll = fmaf(__ldcg(part(i) + RT * DH + RT + n), fast_exp2(mi - mx), ll);
+                        ll = fmaf(__ldcg(part(i) + RT * DH + RT + n), mi == -INFINITY ? 0.f : fast_exp2(mi - mx), ll);
                     }
 #pragma unroll
                     for (int d = 16; d > 0; d >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, d);
@@ -865,8 +866,8 @@ __global__ void __launch_bounds__(kTlThreads, 1)
     #pragma unroll
                             for (int i = 0; i < DH / 16; ++i) {
                                 const uint32_t at = ((uint32_t)(i / 4) * SM::kChunk + (i % 4) * 32) >> 4;
-                                umma_f16_ss_if(is0, tmem + kTmS + t2 * kTlKeys, qd + (t2 * SM::kTile >> 4) + at, kdj + at, idesc_s,
-                                               i > 0 ? 1u : 0u);
+                                umma_f16_ss_if(is0, tmem + kTmS + t2 * kTlKeys, qd + (t2 * SM::kTile >> 4) + at, kdj + at,
+                                               idesc_s, i > 0 ? 1u : 0u);
                             }
                             umma_commit_if(is0, s_full + t2);
                         }
@@ -921,7 +922,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
             fence_proxy_async_smem();
             __syncwarp();
         };
-        // K of block n + 1 goes before V of block n: K has two buffers, so it is ready while the matrix unit is still at block n
+        // K of block n + 1 goes before V of block n: K has two buffers, so it is ready while the matrix unit is at block n
         auto keys = [&](uint32_t i) {
             const uint32_t st = i & 1;
             mbar_wait(c_full + st, i >> 1 & 1, abort, a.err);
@@ -1266,8 +1267,8 @@ int sh_cuda_attention_kv8(uint64_t q, uint64_t o, const sh_cuda_kv8_t *c, uint64
         return -1;
     }
     if (R == 0 || T == 0) return 0;
-    if (!q || !o || !table || !lens || !q_start || ((q | o) & 1)) {
-        sh::set_error(-1, "[sh_cuda_attention_kv8] null array, or odd q / o");
+    if (!q || !o || !table || !lens || !q_start || ((q | o) & 1) || !sh::words_ok(table, lens, q_start)) {
+        sh::set_error(-1, "[sh_cuda_attention_kv8] a null or misaligned array");
         return -1;
     }
     const sh::DeviceState &s = sh::state();
@@ -1302,8 +1303,9 @@ int sh_cuda_attention_kv8(uint64_t q, uint64_t o, const sh_cuda_kv8_t *c, uint64
     if ((uint64_t)max_q * a.G > 64) {
         a.flip = scale < 0.f ? 0x80008000u : 0u;
         a.sl2 = fabsf(a.sl2);
-        if (c->dh == 64) e = fp8 ? launch_tiles<64, true>(a, mk, mv, sms, s.stream) : launch_tiles<64, false>(a, mk, mv, sms, s.stream);
-        else e = fp8 ? launch_tiles<128, true>(a, mk, mv, sms, s.stream) : launch_tiles<128, false>(a, mk, mv, sms, s.stream);
+        auto launch = c->dh == 64 ? (fp8 ? launch_tiles<64, true> : launch_tiles<64, false>)
+                                  : (fp8 ? launch_tiles<128, true> : launch_tiles<128, false>);
+        e = launch(a, mk, mv, sms, s.stream);
     } else if (c->dh == 64) e = wide ? SH_KV8(64, 2, 4) : few ? SH_KV8(64, 1, 8) : SH_KV8(64, 1, 4);
     else e = wide ? SH_KV8(128, 2, 4) : few ? SH_KV8(128, 1, 8) : SH_KV8(128, 1, 4);
 #undef SH_KV8

@@ -6,8 +6,8 @@
 // Bound by the weights' bytes (half a byte per element, read once), and close behind by the instructions that turn codes
 // into operands, so there are two forms of the inner product, both exact but for fp32 sums:
 //   fp16   code - zero is a small integer, exact in fp16: the 16-row operand of the matrix instruction (16 columns of W x
-//          16 k), 8 rows of X its columns, twice for up to 16 rows. 9 instructions turn a word into 8 operands (fp16 patterns 1024 + c and
-//          1024 + 16 c, then one subtraction or FMA).
+//          16 k), 8 rows of X its columns, twice for up to 16 rows. 9 instructions turn a word into 8 operands (fp16
+//          patterns 1024 + c and 1024 + 16 c, then one subtraction or FMA).
 //   int8   for a single row and many columns: every finite fp16 value is an integer times 2^-24 below 2^41, i.e. six signed
 //          base-256 digits. The codes are int8 operands as they are (3 instructions per 8), the digits of X are six of the
 //          instruction's eight columns, of which a single row would leave seven empty, and the int32 sums of a group are
@@ -140,7 +140,8 @@ __host__ __device__ inline W4Layout w4_layout(uint32_t ng, uint32_t d, uint32_t 
     return l;
 }
 
-// INT: digits (M == 1); NT: groups of 8 columns of the matrix instruction; NG: groups of 8 warps; D: stages; Z: zero points given
+// INT: digits (M == 1); NT: groups of 8 columns of the matrix instruction; NG: groups of 8 warps; D: stages; Z: zero points
+// given
 template <int G, bool INT, int NT, int NG, int D, bool Z>
 __global__ void __launch_bounds__(NG * kGroupThreads, 1)
     k_gemv_w4(const __grid_constant__ CUtensorMap mw, W4Args a, uint32_t splits, uint32_t tiles, uint32_t iters) {
@@ -183,7 +184,8 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
         if (p_tile >= tiles) return;
         if (lane == 0) {
             mbar_arrive_expect_tx(full + p_slot, kStage);
-            tma_load_2d(ring + p_slot * kStage, &mw, full + p_slot, (int)((u0 + nu - p_left) * (kUnit / 2)), (int)(p_tile * kRows));
+            tma_load_2d(ring + p_slot * kStage, &mw, full + p_slot, (int)((u0 + nu - p_left) * (kUnit / 2)),
+                        (int)(p_tile * kRows));
         }
         p_slot = p_slot + 1 == D ? 0 : p_slot + 1;
         if (--p_left == 0) p_left = nu, p_tile += tile_step;
@@ -481,7 +483,10 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
         if (NT > 1) group_sync();
     }
     if (*abort)      // a copy did not arrive in time: give those in flight as long again
+    {
         for (int d = 0; d < D; ++d) drain_wait(full + d, phase ^ (d < (int)slot));
+        for (uint32_t i = iter > 2 ? iter - 2 : 0; a.staged && i < iter; ++i) drain_wait(sc_full + (i & 1), i >> 1 & 1);
+    }
     if (splits > 1) {
         cluster_sync_all();
         iter = 0;
@@ -593,8 +598,9 @@ int sh_cuda_gemv_w4(uint64_t x, uint64_t codes, uint64_t scales, uint64_t zeros,
     if (M == 0 || N == 0) return 0;
     if (M > 32 || (group != 32 && group != 64 && group != 128) || K == 0 || K > kMaxK || K % group || ldx < K || ldz < N ||
         (uint64_t)ldw * 2 < K || ldw % 16 || N >= (1u << 31) - 64) {
-        sh::set_error(-1, "[sh_cuda_gemv_w4] need M <= 32, group 32, 64 or 128, K %% group == 0, K <= 262144, ldw %% 16 == 0 (M=%u N=%u K=%u "
-                      "group=%u ldx=%u ldw=%u ldz=%u)", M, N, K, group, ldx, ldw, ldz);
+        sh::set_error(-1, "[sh_cuda_gemv_w4] need M <= 32, group 32, 64 or 128, K %% group == 0, K <= 262144, ldx >= K, ldz >= N, "
+                      "ldw >= K / 2, ldw %% 16 == 0 (M=%u N=%u K=%u group=%u ldx=%u ldw=%u ldz=%u)", M, N, K, group, ldx, ldw,
+                      ldz);
         return -1;
     }
     if (!x || !codes || !scales || !z || !sh::aligned16(codes) || ((x | scales | z) & 1) ||

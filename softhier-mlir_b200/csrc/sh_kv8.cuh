@@ -8,6 +8,9 @@ namespace sh {
 inline bool kv8_page_ok(uint32_t page) { return page == 16 || page == 32 || page == 64 || page == 128; }
 inline uint32_t kv8_shift(uint32_t page) { return page == 16 ? 4u : page == 32 ? 5u : page == 64 ? 6u : 7u; }
 
+// arrays of 32-bit words lie on whole words
+inline bool words_ok(uint64_t a, uint64_t b = 0, uint64_t c = 0, uint64_t d = 0) { return ((a | b | c | d) & 3) == 0; }
+
 // 0, or -1 / -3 with the reason recorded
 inline int kv8_check(const sh_cuda_kv8_t *c, const char *who) {
     if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale || !aligned16(c->k) || !aligned16(c->v) ||

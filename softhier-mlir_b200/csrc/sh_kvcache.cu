@@ -148,8 +148,9 @@ __global__ void __launch_bounds__(kTabThreads) k_kv_tables(TablesArgs a) {
             if (fresh[j] && in == 0) *entry[j] = pid[j];
         }
         if (PER == 4 && a.vec && i0 + PER <= a.t_cap) {
-            *reinterpret_cast<int4 *>(a.slots + i0) = make_int4(slot[0], slot[PER > 1 ? 1 : 0], slot[PER > 2 ? 2 : 0], slot[PER - 1]);
-            *reinterpret_cast<int4 *>(a.pos + i0) = make_int4(pos[0], pos[PER > 1 ? 1 : 0], pos[PER > 2 ? 2 : 0], pos[PER - 1]);
+            constexpr uint32_t j1 = PER > 1 ? 1 : 0, j2 = PER > 2 ? 2 : 0;
+            *reinterpret_cast<int4 *>(a.slots + i0) = make_int4(slot[0], slot[j1], slot[j2], slot[PER - 1]);
+            *reinterpret_cast<int4 *>(a.pos + i0) = make_int4(pos[0], pos[j1], pos[j2], pos[PER - 1]);
         } else {
 #pragma unroll
             for (uint32_t j = 0; j < PER; ++j)
@@ -462,9 +463,11 @@ int sh_cuda_kv_tables(uint64_t lens, uint64_t add, uint32_t R, uint32_t page, ui
         return -1;
     }
     if (R && (!lens || !add || !table || !ring || !pool || !pool_out || !lens_out || !q_start || ld_table == 0 ||
-              ld_table >= (1u << 31) / page || (t_cap && (!slots || !pos)) || t_cap >= (1u << 31))) {
-        sh::set_error(-1, "[sh_cuda_kv_tables] a null array, or ld_table * page or t_cap past 2^31 (ld_table=%u t_cap=%u)",
-                      ld_table, t_cap);
+              ld_table >= (1u << 31) / page || (t_cap && (!slots || !pos)) || t_cap >= (1u << 31) ||
+              !sh::words_ok(lens, add, table, ring) || !sh::words_ok(pool, pool_out, lens_out, q_start) ||
+              !sh::words_ok(slots, pos))) {
+        sh::set_error(-1, "[sh_cuda_kv_tables] a null or misaligned array, or ld_table * page or t_cap past 2^31 (ld_table=%u "
+                      "t_cap=%u)", ld_table, t_cap);
         return -1;
     }
     if (R == 0) return 0;
@@ -490,9 +493,9 @@ int sh_cuda_kv8_append(const sh_cuda_kv8_t *c, uint64_t k, uint64_t v, uint32_t 
     const int bad = sh::kv8_check(c, "sh_cuda_kv8_append");
     if (bad) return bad;
     const uint64_t w = (uint64_t)c->heads * c->dh;
-    if (T && (!k || !v || !slots || (k & 1) || (v & 1) || ldk < w || ldv < w || T >= (1u << 31))) {
-        sh::set_error(-1, "[sh_cuda_kv8_append] null or odd k / v, null slots, or ldk, ldv < heads * dh (ldk=%u ldv=%u)",
-                      ldk, ldv);
+    if (T && (!k || !v || !slots || ((k | v) & 1) || !sh::words_ok(slots) || ldk < w || ldv < w || T >= (1u << 31))) {
+        sh::set_error(-1, "[sh_cuda_kv8_append] null or odd k / v, null or misaligned slots, or ldk, ldv < heads * dh (ldk=%u "
+                      "ldv=%u)", ldk, ldv);
         return -1;
     }
     if (T == 0) return 0;
@@ -500,8 +503,8 @@ int sh_cuda_kv8_append(const sh_cuda_kv8_t *c, uint64_t k, uint64_t v, uint32_t 
     AppendArgs a = {{(uint8_t *)c->k, (uint8_t *)c->v}, {(float *)c->k_scale, (float *)c->v_scale},
                     {(const __half *)k, (const __half *)v}, {ldk, ldv}, (const int *)slots, c->page_stride, T, c->pages,
                     sh::kv8_shift(c->page), c->heads, 0, s.dev_err};
-    // A prompt's pages hold up to `page` new rows each: 64 rows per CTA and at least a page (4096 tokens, 8 heads of 64, pages of
-    // 16: 9 us, 21 us with 16 rows). Few rows are mostly one per page: eight rows per CTA spread them over the GPU, 16 in
+    // A prompt's pages hold up to `page` new rows each: 64 rows per CTA and at least a page (4096 tokens, 8 heads of 64,
+    // pages of 16: 9 us, 21 us with 16 rows). Few rows are mostly one per page: eight rows per CTA spread them over the GPU, 16 in
     // between (1024 rows 4.9 us, 6.2 us with eight).
     const uint32_t many = c->page > 64 ? c->page : 64;
     const uint64_t ctas = (uint64_t)((T + many - 1) / many) * c->heads * 2;

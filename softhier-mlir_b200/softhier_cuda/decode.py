@@ -51,6 +51,8 @@ class KvCache:
 
     def step(self, add: torch.Tensor) -> None:
         """add: int32 [requests] on the device, tokens of each request in this step (< 0: it has ended)."""
+        if add.dtype != torch.int32 or add.shape != self.lens.shape or add.device != self.lens.device or not add.is_contiguous():
+            raise ShCudaError(f"add is not a contiguous int32 [{self.requests}] on {self.lens.device}")
         p = torch.Tensor.data_ptr
         self._must(self.rt.lib.sh_cuda_kv_tables(
             p(self.lens), p(add), self.requests, self.page, p(self.table), self.blocks, p(self.ring), self.pages,
@@ -78,6 +80,8 @@ def quantize_w4(w: np.ndarray, group: int, symmetric: bool = False):
     if group not in (32, 64, 128) or K % group:
         raise ValueError(f"K {K} is not a multiple of a group of 32, 64 or 128 ({group})")
     x = np.ascontiguousarray(np.asarray(w, np.float32).T).reshape(N, K // group, group)
+    if not np.abs(x).max(initial=0.0) <= 65504.0:
+        raise ValueError("a weight is not finite or beyond fp16")
     if symmetric:
         scales = (np.abs(x).max(2) / 7.0).astype(np.float16)
         zeros = None

@@ -60,12 +60,14 @@ def test_other_formats_are_refused(lib, capfd):
 def test_append_and_attention_refusals(lib, capfd):
     lib.sh_cuda_last_error()
     for args in ((0, A, 1, 256, 256, A), (A, 0, 1, 256, 256, A), (A, A, 1, 255, 256, A), (A, A, 1, 256, 255, A),
-                 (A, A, 1, 256, 256, 0), (A + 1, A, 1, 256, 256, A), (A, A, 1 << 31, 256, 256, A)):
+                 (A, A, 1, 256, 256, 0), (A + 1, A, 1, 256, 256, A), (A, A, 1 << 31, 256, 256, A),
+                 (A, A, 1, 256, 256, A + 2)):
         assert lib.sh_cuda_kv8_append(_cache(), *args) == -1, args
     assert lib.sh_cuda_kv8_append(_cache(), 0, 0, 0, 256, 256, 0) == 0           # no rows: nothing to do
     for kw in (dict(H=6), dict(H=0), dict(ldq=511), dict(ldo=511), dict(q=0), dict(o=0), dict(q=A + 1), dict(table=0),
                dict(lens=0), dict(q_start=0), dict(ld_table=0), dict(ld_table=1 << 27), dict(scale=float("nan")),
-               dict(scale=float("inf")), dict(ws=0), dict(ws=A + 4), dict(ws_bytes=L.KV8_WS_BYTES - 1), dict(T=1 << 29)):
+               dict(scale=float("inf")), dict(ws=0), dict(ws=A + 4), dict(ws_bytes=L.KV8_WS_BYTES - 1), dict(T=1 << 29),
+               dict(table=A + 2), dict(lens=A + 1), dict(q_start=A + 3)):
         assert _attn(lib, _cache(), **kw) == -1, kw
     assert _attn(lib, _cache(), R=0) == 0 and _attn(lib, _cache(), T=0) == 0
     lib.sh_cuda_last_error()
@@ -78,7 +80,8 @@ def test_tables_refusals(lib, capfd):
                 slots=A, pos=A, t_cap=64)
     for kw in (dict(page=8), dict(page=0), dict(page=48), dict(pages=0), dict(pages=1 << 27), dict(R=8193), dict(lens=0),
                dict(add=0), dict(table=0), dict(ring=0), dict(pool=0), dict(pool_out=0), dict(lens_out=0), dict(q_start=0),
-               dict(slots=0), dict(pos=0), dict(ld_table=0), dict(ld_table=1 << 27), dict(t_cap=1 << 31)):
+               dict(slots=0), dict(pos=0), dict(ld_table=0), dict(ld_table=1 << 27), dict(t_cap=1 << 31),
+               *({name: A + 2} for name in good if good[name] == A)):
         assert lib.sh_cuda_kv_tables(*(good | kw).values()) == -1, kw
     assert lib.sh_cuda_kv_tables(*(good | dict(R=0)).values()) == 0
     assert "[sh_cuda_kv_tables]" in capfd.readouterr().out
@@ -89,7 +92,8 @@ def test_gemv_w4_refusals(lib, capfd):
     lib.sh_cuda_last_error()
     good = dict(x=A, codes=A, scales=A, zeros=0, z=A, M=4, N=64, K=256, ldx=256, ldw=128, ldz=64, group=64, bias=0, residual=0,
                 ldr=0, flags=0)
-    for kw in (dict(M=33), dict(group=16), dict(group=256), dict(K=224), dict(K=0), dict(K=(1 << 18) + 64, ldx=1 << 20, ldw=1 << 19), dict(ldx=255), dict(ldz=63), dict(ldw=112),
+    for kw in (dict(M=33), dict(group=16), dict(group=256), dict(K=224), dict(K=0),
+               dict(K=(1 << 18) + 64, ldx=1 << 20, ldw=1 << 19), dict(ldx=255), dict(ldz=63), dict(ldw=112),
                dict(ldw=136), dict(x=0), dict(codes=0), dict(codes=A + 8), dict(scales=0), dict(z=0), dict(x=A + 1),
                dict(flags=L.EPI_BIAS), dict(flags=L.EPI_RESIDUAL), dict(flags=L.EPI_RESIDUAL, residual=A, ldr=63),
                dict(flags=L.EPI_GELU), dict(flags=L.EPI_ACCUMULATE)):
@@ -116,6 +120,10 @@ def test_quantize_w4_is_within_a_step(group, symmetric):
     assert np.all(back[:group, 3] == 0)
     with pytest.raises(ValueError):
         decode.quantize_w4(w, 96)
+    for x in (np.nan, np.inf, 1e7):                        # no fp16 scale
+        w[5, 5] = x
+        with pytest.raises(ValueError):
+            decode.quantize_w4(w, group, symmetric)
 
 
 def test_oracle_e4m3_agrees_with_torch():

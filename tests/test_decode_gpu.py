@@ -10,6 +10,7 @@ import torch
 
 from oracle import decode as D, llm
 from softhier_cuda import decode, lib as L
+from softhier_cuda.runtime import ShCudaError
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -774,6 +775,17 @@ def test_a_decode_loop(gpu_lib, fmt, captured):
         else:
             step(8, 1)
         check(before, adds, 8)
+
+
+def test_cache_refuses_other_step_tensors(gpu_lib):
+    cache = decode.KvCache(gpu_lib, layers=1, heads=2, dh=64, page=16, pages=8, requests=3, blocks=2)
+    for add in (torch.ones(3, dtype=torch.int64, device=DEV), _i32([1, 1]), torch.ones(3, dtype=torch.int32),
+                _i32([1, 1, 1, 1, 1, 1])[::2]):
+        with pytest.raises(ShCudaError):
+            cache.step(add)
+    with pytest.raises(ShCudaError):
+        cache.append(0, 256, 256, 128, 128, 4)      # more rows than a step has
+    assert _np(cache.pool).tolist()[:2] == [0, 8]
 
 
 def test_two_streams_with_their_own_workspaces(gpu_lib):
