@@ -578,32 +578,55 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
             if (s_flag) {
                 const uint32_t parts = c1 - c0 + 1;
                 auto part = [&](uint32_t i) { return a.part + (size_t)(2 * (c0 + i) + (i == 0)) * RT * (DH + 2); };
-                // each row's maximum and sum, one warp per row
-                for (uint32_t n = warp; n < nrows; n += NW) {
+                // Each row's maximum and sum: eight lanes per row, eight parts of each in flight.
+                constexpr uint32_t kAhead = 8;
+                for (uint32_t n = t >> 3; n < (nrows + 3) / 4 * 4; n += kThreads / 8) {      // whole warps: shuffles
                     float mx = -INFINITY, ll = 0.f;
-                    for (uint32_t i = lane; i < parts; i += 32) mx = fmaxf(mx, __ldcg(part(i) + RT * DH + n));
+                    for (uint32_t i0 = t & 7; i0 < parts; i0 += 8 * kAhead) {
+                        float mi[kAhead], li[kAhead], mb = mx;
 #pragma unroll
-                    for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                    for (uint32_t i = lane; i < parts; i += 32) {
-                        const float mi = __ldcg(part(i) + RT * DH + n);
-                        ll = fmaf(__ldcg(part(i) + RT * DH + RT + n), mi == -INFINITY ? 0.f : fast_exp2(mi - mx), ll);
+                        for (uint32_t q = 0; q < kAhead; ++q) {
+                            const bool in = n < nrows && i0 + 8 * q < parts;
+                            mi[q] = in ? __ldcg(part(i0 + 8 * q) + RT * DH + n) : -INFINITY;
+                            li[q] = in ? __ldcg(part(i0 + 8 * q) + RT * DH + RT + n) : 0.f;
+                        }
+#pragma unroll
+                        for (uint32_t q = 0; q < kAhead; ++q) mb = fmaxf(mb, mi[q]);
+                        ll *= mx == -INFINITY ? 1.f : fast_exp2(mx - mb);
+                        mx = mb;
+#pragma unroll
+                        for (uint32_t q = 0; q < kAhead; ++q)
+                            ll = fmaf(li[q], mi[q] == -INFINITY ? 0.f : fast_exp2(mi[q] - mx), ll);
                     }
+                    __syncwarp();
+                    float mt = mx;
 #pragma unroll
-                    for (int d = 16; d > 0; d >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, d);
-                    if (lane == 0) s_m[n] = mx, s_l[n] = ll;
+                    for (int d = 4; d > 0; d >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, d));
+                    ll *= mx == -INFINITY ? 1.f : fast_exp2(mx - mt);
+#pragma unroll
+                    for (int d = 4; d > 0; d >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, d);
+                    if ((t & 7) == 0 && n < nrows) s_m[n] = mt, s_l[n] = ll;
                 }
                 __syncthreads();
                 for (uint32_t e = t; e < nrows * (DH / 2); e += kThreads) {
                     const uint32_t n = e / (DH / 2), j = e % (DH / 2), d = (j & 7) * VB + (j >> 3) * 2;
                     const float mx = s_m[n], ll = s_l[n];
                     float x = 0.f, y = 0.f;
-#pragma unroll 8
-                    for (uint32_t i = 0; i < parts; ++i) {
-                        const float *pi = part(i);
-                        const float mi = __ldcg(pi + RT * DH + n);
-                        const float2 z = __ldcg(reinterpret_cast<const float2 *>(pi + n * DH + 2 * j));
-                        const float f = mi == -INFINITY ? 0.f : fast_exp2(mi - mx);
-                        x = fmaf(z.x, f, x), y = fmaf(z.y, f, y);
+                    for (uint32_t i0 = 0; i0 < parts; i0 += kAhead) {
+                        float f[kAhead];
+                        float2 z[kAhead];
+#pragma unroll
+                        for (uint32_t q = 0; q < kAhead; ++q) {
+                            const float *pi = part(min(i0 + q, parts - 1));
+                            f[q] = __ldcg(pi + RT * DH + n);
+                            z[q] = __ldcg(reinterpret_cast<const float2 *>(pi + n * DH + 2 * j));
+                        }
+#pragma unroll
+                        for (uint32_t q = 0; q < kAhead; ++q) {
+                            if (i0 + q >= parts) continue;
+                            f[q] = f[q] == -INFINITY ? 0.f : fast_exp2(f[q] - mx);
+                            x = fmaf(z[q].x, f[q], x), y = fmaf(z[q].y, f[q], y);
+                        }
                     }
                     write_out(n, d, x, y, ll);
                 }
