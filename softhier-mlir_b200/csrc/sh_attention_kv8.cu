@@ -7,7 +7,7 @@
 // (int8 and e4m3 are exact in fp16) are the operands of the second product. The first product is exact up to its
 // fp32 sums. The sum of the weights is taken in fp32; for the second product they are fp16 operands, in the kernel for few
 // rows with the rest of that rounding as a second operand (the outputs' own rounding is then all there is; it costs 5 of the
-// 114 us of a large batch), in the one for many rows without it (2^-11 relative, as the outputs' own).
+// 115 us of a large batch), in the one for many rows without it (2^-11 relative, as the outputs' own).
 #include <math.h>
 
 #include "sh_kv8.cuh"
@@ -25,6 +25,8 @@ struct KvArgs {
     float sl2;            // scale * log2(e)
     uint32_t vec;         // q rows take 16-byte loads, o rows 4-byte stores
     uint32_t vec_o;       // o rows take 16-byte stores
+    uint32_t box_step, k_at, v_at;      // few rows: bytes from 16 tokens to the next in a stage, K's and V's place there
+    uint32_t boxes, box_bytes;          // few rows: copies per step
     uint32_t flip;        // sign bits to turn in q: the scale is negative (sl2 is its magnitude then; tiles only)
     uint32_t *counters;   // arrivals per CTA whose last item goes on in others, zero between calls
     float *part;
@@ -60,6 +62,12 @@ __device__ __forceinline__ uint2 lds8(uint32_t at) {
 // 4 bytes to shared memory, counted on `bar` with this thread's other copies by cp_async_arrive
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void *src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+// a box of a K and V map (below)
+__device__ __forceinline__ void tma_load_pair(void *dst, const CUtensorMap *map, uint64_t *bar, int row, int page) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %3}], [%2];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(0), "r"(row), "r"(page)
+                 : "memory");
 }
 __device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -129,12 +137,15 @@ __device__ __forceinline__ uint32_t byte_pair(uint32_t a, uint32_t b) {
 // both operands agree: a lane takes 16 neighbouring columns of its K rows, and 4 tokens of V with dh / 8 neighbouring
 // columns. W^T comes from S^T by an 8 x 8 transpose in registers.
 //
-// A warp takes 16 tokens of a unit at dh = 128, 32 at dh = 64 (as many bytes); its K and V boxes (16 rows, swizzled so that
-// neither operand's reads meet in a bank more than two at a time) come by TMA into a ring of its own, kStages ahead and
-// across items, so a warp waits for nobody but its own copies until an item ends. What bounds it beside the bytes is the
-// integer pipe: turning int8 codes into fp16 operands takes 112 of its instructions per 16 tokens and warp at dh = 128, 56 of
-// the 157 cycles that their bytes take, and the rest of a step as much again. The copies alone (no products) run at 0.87 of
-// the measured copy rate.
+// A warp takes 16 tokens of a unit at dh = 128, 32 at dh = 64 (as many bytes); its K and V boxes, both with one instruction
+// (swizzled so that neither operand's reads meet in a bank more than two at a time), come by TMA into a ring of its own,
+// kStages ahead and across items, so a warp waits for nobody but its own copies until an item ends. The scales come in
+// registers as far ahead. What bounds it beside the bytes is the integer pipe: turning int8 codes into fp16 operands takes 112
+// of its instructions per 16 tokens and warp at dh = 128, 56 of the 157 cycles that their bytes take, and the rest of a step
+// as much again. 64 requests of up to 8192 tokens (32 heads over 8 of 128, int8) take 115 us, the copies alone (no products) 98;
+// with heads of 64 (15 over 5) 53 and 39. More warps per SM (20 at dh = 64) are slower. Drafts add what an item's end
+// costs: up to 16 rows of partial sums per warp and CTA. Their dh = 128 form has 8 warps per SM with all of their registers
+// (32 requests of 4 drafts 70 us; with 12 warps, which spill, 75).
 //
 // Work is split evenly whatever the lengths are: the units (request, kv head, row tile, block of tokens), in this order,
 // are dealt to the CTAs in equal contiguous runs, which every CTA works out from the lengths by itself. An item (request,
@@ -181,20 +192,20 @@ struct RowsSmem {
     static constexpr uint32_t kTokens = 2048 / DH;                    // of a step: 16 or 32
     static constexpr uint32_t kTile = kTokens * DH;                   // K or V of a step
     static constexpr uint32_t kRing = 0, kO = NW * kStages * 2 * kTile, kM = kO + NW * 8 * NT * (DH + 4) * 4;
-    static constexpr uint32_t kL = kM + NW * 8 * NT * 4, kScale = kL + NW * 8 * NT * 4;     // {ks, vs, usable} per 16 tokens
-    static constexpr uint32_t kBars = kScale + NW * kStages * 32, kPart = kBars + NW * kStages * 8;
+    static constexpr uint32_t kL = kM + NW * 8 * NT * 4, kBars = kL + NW * 8 * NT * 4, kPart = kBars + NW * kStages * 8;
     static constexpr uint32_t kMisc = kPart + NW * 8, kBytes = kMisc + 64 + 1024;
 };
 
 template <int DH, int NT, int NW, bool FP8>
-__global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
-    k_attn_kv8_rows(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, KvArgs a) {
+__global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : DH == 64 ? 12 : 8) / NW)
+    k_attn_kv8_rows(const __grid_constant__ CUtensorMap mkv, KvArgs a) {
     using SM = RowsSmem<DH, NT, NW>;
     constexpr uint32_t RT = 8 * NT, kThreads = NW * 32;                     // rows of a tile
     constexpr uint32_t kStep = SM::kTokens, kKeys = kStep * NW;             // keys of a warp's step, of a unit
     constexpr int KC = DH / 64;                     // 16-byte pieces of a K row per lane
     constexpr int VB = DH / 8;                      // V columns per lane
     constexpr int VW = VB / 4;                      // as words
+    constexpr uint32_t HF = kStep / 16;             // groups of 16 tokens of a step, each in one page
     extern __shared__ uint8_t smem_raw[];
     uint8_t *sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     // [NW][RT] rows of DH / 2 column pairs: pair i of lane row g (columns VB g + 2 i) at i * 8 + g, so that neither the writes
@@ -216,8 +227,8 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
     const uint32_t page1 = (1u << a.page_shift) - 1;
     uint64_t *full = reinterpret_cast<uint64_t *>(sm + SM::kBars) + warp * kStages;
     if (lane == 0)
-        for (int i = 0; i < kStages; ++i) mbar_init(full + i, 2);
-    if (t == 0) *abort = 0, prefetch_tmap(&mk), prefetch_tmap(&mv);
+        for (int i = 0; i < kStages; ++i) mbar_init(full + i, 1);
+    if (t == 0) *abort = 0, prefetch_tmap(&mkv);
     fence_mbar_init();
     fence_proxy_async_smem();
     pdl_launch_dependents();
@@ -267,7 +278,6 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
     // ---- the copies run ahead of the sums: cursor `p`. Lane i holds the page of the unit that is i units further in p's item
     // than `p_base`; the table is read again, a step before it is needed, when the item or the 32 units end. -----------
     const uint32_t ring = smem_u32(sm) + SM::kRing + warp * (kStages * 2 * SM::kTile);
-    uint8_t *s_scale = sm + SM::kScale + warp * (kStages * 32);
     Cursor k;
     k.r = s_start.r, k.v = s_start.v;
     cursor_sizes<RT, kKeys>(k, a);
@@ -280,13 +290,12 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
     u64 p_left = end - begin;
     // the warp's tokens of the cursor's unit hold keys
     auto in_use = [&](const Cursor &x) { return (int)(x.b * kKeys + warp * kStep) < x.lim_hi; };
-    constexpr int HF = kStep / 16;      // groups of 16 tokens, each in one page
     uint32_t p_base = k.b;
     int p_ids[HF];
     auto lookup = [&]() {
         p_base = p.b;
 #pragma unroll
-        for (int f = 0; f < HF; ++f) {
+        for (uint32_t f = 0; f < HF; ++f) {
             const uint32_t tok = (p.b + lane) * kKeys + warp * kStep + f * 16;
             p_ids[f] = p_left && (int)tok < p.lim_hi ? a.table[(size_t)p.r * a.ld_table + (tok >> a.page_shift)] : -1;
         }
@@ -298,43 +307,48 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
         if (p.b == 0 || p.b - p_base == 32) lookup();
     };
     uint32_t p_slot = 0;
+    float2 scales[2][HF];      // of the two units on their way, the nearer first; {.., -1}: left out
+#pragma unroll
+    for (uint32_t f = 0; f < HF; ++f) scales[0][f] = scales[1][f] = make_float2(0.f, -1.f);
     auto issue = [&]() {      // the next unit in which this warp has keys
         while (p_left && !in_use(p)) advance();
-        if (p_left == 0) return;
+        if (p_left == 0) {
+#pragma unroll
+            for (uint32_t f = 0; f < HF; ++f) scales[0][f] = scales[1][f];
+            return;
+        }
         int id[HF];
 #pragma unroll
-        for (int f = 0; f < HF; ++f) id[f] = __shfl_sync(0xffffffffu, p_ids[f], p.b - p_base);
-        if (lane == 0) {
-            constexpr uint32_t kBox = SM::kTile / HF;
-            const uint32_t tok = p.b * kKeys + warp * kStep;
-            uint64_t *bar = full + p_slot;
-            uint8_t *dst = sm + SM::kRing + (warp * kStages + p_slot) * (2 * SM::kTile);
-            int *info = reinterpret_cast<int *>(s_scale + p_slot * 32);
-            uint32_t boxes = 0;
+        for (uint32_t f = 0; f < HF; ++f) id[f] = __shfl_sync(0xffffffffu, p_ids[f], p.b - p_base);
+        const uint32_t tok = p.b * kKeys + warp * kStep;
 #pragma unroll
-            for (int f = 0; f < HF; ++f) boxes += (uint32_t)id[f] < a.pages;
-            mbar_arrive_expect_tx(bar, boxes * 2 * kBox);
-#pragma unroll
-            for (int f = 0; f < HF; ++f) {
-                const bool good = (uint32_t)id[f] < a.pages;
-                info[4 * f + 2] = good;
-                if (good) {
-                    const int row = (int)((p.kvh << a.page_shift) + ((tok + f * 16) & page1));
-                    const size_t at = (size_t)id[f] * a.heads + p.kvh;
-                    tma_load_3d(dst + f * kBox, &mk, bar, 0, row, id[f]);
-                    tma_load_3d(dst + SM::kTile + f * kBox, &mv, bar, 0, row, id[f]);
-                    cp_async4(smem_u32(info + 4 * f), a.ks + at);
-                    cp_async4(smem_u32(info + 4 * f) + 4, a.vs + at);
-                } else if ((int)tok + f * 16 < p.lim_hi) {
-                    atomicCAS(a.err, 0, (int)sh::kErrBadArgs);
-                }
+        for (uint32_t f = 0; f < HF; ++f) {
+            scales[0][f] = scales[1][f];
+            scales[1][f] = make_float2(0.f, -1.f);
+            if ((uint32_t)id[f] < a.pages) {
+                const size_t at = (size_t)id[f] * a.heads + p.kvh;
+                scales[1][f] = make_float2(__ldg(a.ks + at), __ldg(a.vs + at));
+            } else if ((int)(tok + f * 16) < p.lim_hi && lane == 0) {
+                atomicCAS(a.err, 0, (int)sh::kErrBadArgs);
             }
-            cp_async_arrive(bar);
+        }
+        if (lane == 0) {
+            uint64_t *bar = full + p_slot;
+            uint32_t n = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < HF; ++i) n += i < a.boxes && (uint32_t)id[i] < a.pages;
+            mbar_arrive_expect_tx(bar, n * a.box_bytes);
+#pragma unroll
+            for (uint32_t i = 0; i < HF; ++i)
+                if (i < a.boxes && (uint32_t)id[i] < a.pages)
+                    tma_load_pair(sm + SM::kRing + (warp * kStages + p_slot) * (2 * SM::kTile) + i * SM::kTile, &mkv, bar,
+                                  (int)((p.kvh << a.page_shift) + ((tok + i * 16) & page1)), id[i]);
         }
         p_slot = p_slot + 1 == kStages ? 0 : p_slot + 1;
         advance();
     };
     for (int i = 0; i < kStages; ++i) issue();
+    __syncwarp();
     uint32_t slot = 0, phase = 0;
 
     for (u64 u = begin; u < end;) {
@@ -348,37 +362,49 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
         // ---- Q as the column operand: lane (g, c) holds columns 16 c .. of row 8 nt + g ------------------------------
         uint32_t qf[NT][KC * 4][2];
         int lim[NT][2];
+        {
+            uint32_t w[NT][KC][8];      // all loads before the first use
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const uint32_t n = nt * 8 + g;
-            const uint32_t rr = row0 + n, qi = rr / a.G, gi = rr - qi * a.G;
-            const __half *qp = a.q + (size_t)(v.qs + qi) * a.ldq + ((size_t)kvh * a.G + gi) * DH + c * 16;
+            for (int nt = 0; nt < NT; ++nt) {
+                const uint32_t n = nt * 8 + g, rr = row0 + n, qi = rr / a.G, gi = rr - qi * a.G;
+                const __half *qp = a.q + (size_t)(v.qs + qi) * a.ldq + ((size_t)kvh * a.G + gi) * DH + c * 16;
 #pragma unroll
-            for (int j = 0; j < KC; ++j) {
-                uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                if (n < nrows) {
+                for (int j = 0; j < KC; ++j) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[nt][j][e] = 0;
+                    if (n >= nrows) continue;
                     if (a.vec) {
-                        *reinterpret_cast<uint4 *>(w) = *reinterpret_cast<const uint4 *>(qp + j * 64);
-                        *reinterpret_cast<uint4 *>(w + 4) = *reinterpret_cast<const uint4 *>(qp + j * 64 + 8);
+                        const uint4 x = *reinterpret_cast<const uint4 *>(qp + j * 64);
+                        const uint4 y = *reinterpret_cast<const uint4 *>(qp + j * 64 + 8);
+                        w[nt][j][0] = x.x, w[nt][j][1] = x.y, w[nt][j][2] = x.z, w[nt][j][3] = x.w;
+                        w[nt][j][4] = y.x, w[nt][j][5] = y.y, w[nt][j][6] = y.z, w[nt][j][7] = y.w;
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            w[e >> 1] |= (uint32_t)__half_as_ushort(qp[j * 64 + e]) << (16 * (e & 1));
+                        for (int e = 0; e < 8; ++e)
+                            w[nt][j][e] = (uint32_t)__half_as_ushort(qp[j * 64 + 2 * e]) |
+                                          (uint32_t)__half_as_ushort(qp[j * 64 + 2 * e + 1]) << 16;
                     }
                 }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    // columns 4 i .. 4 i + 3 in the order word_to_h2 gives K's
-                    qf[nt][j * 4 + i][0] = FP8 ? w[2 * i] : __byte_perm(w[2 * i], w[2 * i + 1], 0x5410);
-                    qf[nt][j * 4 + i][1] = FP8 ? w[2 * i + 1] : __byte_perm(w[2 * i], w[2 * i + 1], 0x7632);
-                }
             }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < KC; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        // columns 4 i .. 4 i + 3 in the order word_to_h2 gives K's
+                        const uint32_t x = w[nt][j][2 * i], y = w[nt][j][2 * i + 1];
+                        qf[nt][j * 4 + i][0] = FP8 ? x : __byte_perm(x, y, 0x5410);
+                        qf[nt][j * 4 + i][1] = FP8 ? y : __byte_perm(x, y, 0x7632);
+                    }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const uint32_t m = nt * 8 + 2 * c + e;
                 lim[nt][e] = m < nrows ? min(max(v.base + (int)((row0 + m) / a.G) + 1, 0), ctx) : lim_hi;
             }
-        }
 
         float o[DH / 16][NT][4];
         float m[NT][2], top[NT][2], l[NT][2];      // the maximum (0 before there is one), the maximum + 8, the sum
@@ -395,16 +421,14 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
             if ((int)(b * kKeys + warp * kStep) >= lim_hi) break;
             if (!mbar_try_wait(full + slot, phase)) mbar_wait(full + slot, phase, abort, a.err);
             const uint32_t ring_at = ring + slot * (2 * SM::kTile);
-            const uint8_t *infos = s_scale + slot * 32;
             slot = slot + 1 == kStages ? 0 : slot + 1;
             phase ^= slot == 0;
 #pragma unroll
-            for (int f = 0; f < HF; ++f) {
+            for (uint32_t f = 0; f < HF; ++f) {
                 const int tok0 = (int)(b * kKeys + warp * kStep + f * 16);
-                const float4 info = *reinterpret_cast<const float4 *>(infos + 16 * f);
-                if (__float_as_int(info.z) == 0) continue;      // no keys of this tile, or no such page: left out
-                const uint32_t kt = ring_at + f * 16 * DH, vt = kt + SM::kTile;
-                const float ks = info.x, vs = info.y;
+                const float ks = scales[0][f].x, vs = scales[0][f].y;
+                if (vs < 0.f) continue;      // no keys of this tile, or no such page: left out
+                const uint32_t kt = ring_at + f * a.box_step + a.k_at, vt = ring_at + f * a.box_step + a.v_at;
                 float s[NT][4];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
@@ -533,6 +557,21 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
                     s_o[(warp * RT + n) * kPitch + i * 8 + g] = make_float2(o[i][nt][e], o[i][nt][e + 2]);
             }
         __syncthreads();
+        if (NT > 1) {      // many rows: each one's factors of the warps in place of their maxima, and its sum, once
+            if (t < RT) {
+                float mx = -INFINITY, ll = 0.f;
+#pragma unroll
+                for (uint32_t w = 0; w < NW; ++w) mx = fmaxf(mx, s_m[w * RT + t]);
+#pragma unroll
+                for (uint32_t w = 0; w < NW; ++w) {
+                    const float mw = s_m[w * RT + t], f = mw == -INFINITY ? 0.f : fast_exp2(mw - mx);
+                    ll = fmaf(s_l[w * RT + t], f, ll);
+                    s_m[w * RT + t] = f;
+                }
+                s_l[t] = ll, s_l[RT + t] = mx;
+            }
+            __syncthreads();
+        }
         auto write_out = [&](uint32_t n, uint32_t d, float x, float y, float ll) {
             const float inv = ll == 0.f ? 0.f : 1.f / ll;
             const uint32_t rr = row0 + n, qi = rr / a.G, gi = rr - qi * a.G;
@@ -543,19 +582,24 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
         const bool whole = b0 == 0 && b1 == blocks;
         const uint32_t slot = 2 * blockIdx.x + (b0 == 0 ? 1 : 0);
         float *po = a.part + (size_t)slot * RT * (DH + 2), *pm = po + RT * DH, *pl = pm + RT;
-        for (uint32_t e = t; e < nrows * (DH / 2); e += kThreads) {
-            const uint32_t n = e / (DH / 2), j = e % (DH / 2), d = (j & 7) * VB + (j >> 3) * 2;
-            float mx = -INFINITY;
+        constexpr uint32_t kRowsPer = kThreads / (DH / 2);      // a thread has one column pair of every kRowsPer-th row
+        const uint32_t j = t % (DH / 2), d = (j & 7) * VB + (j >> 3) * 2;
+#pragma unroll(NT > 1 ? 4 : 1)
+        for (uint32_t n = t / (DH / 2); n < nrows; n += kRowsPer) {
+            float mx = NT > 1 ? s_l[RT + n] : -INFINITY, ll = NT > 1 ? s_l[n] : 0.f, x = 0.f, y = 0.f;
+            if (NT == 1)
 #pragma unroll
-            for (uint32_t w = 0; w < NW; ++w) mx = fmaxf(mx, s_m[w * RT + n]);
-            float x = 0.f, y = 0.f, ll = 0.f;
+                for (uint32_t w = 0; w < NW; ++w) mx = fmaxf(mx, s_m[w * RT + n]);
 #pragma unroll
             for (uint32_t w = 0; w < NW; ++w) {
-                const float mw = s_m[w * RT + n], f = mw == -INFINITY ? 0.f : fast_exp2(mw - mx);
+                float f = s_m[w * RT + n];
+                if (NT == 1) {
+                    f = f == -INFINITY ? 0.f : fast_exp2(f - mx);
+                    ll = fmaf(s_l[w * RT + n], f, ll);
+                }
                 const float2 p = s_o[(w * RT + n) * kPitch + j];
                 x = fmaf(p.x, f, x);
                 y = fmaf(p.y, f, y);
-                ll = fmaf(s_l[w * RT + n], f, ll);
             }
             if (whole) {
                 write_out(n, d, x, y, ll);
@@ -578,8 +622,9 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
             if (s_flag) {
                 const uint32_t parts = c1 - c0 + 1;
                 auto part = [&](uint32_t i) { return a.part + (size_t)(2 * (c0 + i) + (i == 0)) * RT * (DH + 2); };
-                // Each row's maximum and sum: eight lanes per row, eight parts of each in flight.
-                constexpr uint32_t kAhead = 8;
+                // eight loads in flight: a single row's parts, or two of four rows
+                constexpr uint32_t kAhead = 8, kR = NT > 1 ? 4 : 1, kP = kAhead / kR;
+                // each row's maximum and sum, by eight lanes
                 for (uint32_t n = t >> 3; n < (nrows + 3) / 4 * 4; n += kThreads / 8) {      // whole warps: shuffles
                     float mx = -INFINITY, ll = 0.f;
                     for (uint32_t i0 = t & 7; i0 < parts; i0 += 8 * kAhead) {
@@ -608,27 +653,37 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : 12) / NW)
                     if ((t & 7) == 0 && n < nrows) s_m[n] = mt, s_l[n] = ll;
                 }
                 __syncthreads();
-                for (uint32_t e = t; e < nrows * (DH / 2); e += kThreads) {
-                    const uint32_t n = e / (DH / 2), j = e % (DH / 2), d = (j & 7) * VB + (j >> 3) * 2;
-                    const float mx = s_m[n], ll = s_l[n];
-                    float x = 0.f, y = 0.f;
-                    for (uint32_t i0 = 0; i0 < parts; i0 += kAhead) {
-                        float f[kAhead];
-                        float2 z[kAhead];
+                for (uint32_t n0 = t / (DH / 2); n0 < nrows; n0 += kR * kRowsPer) {
+                    float x[kR], y[kR];
 #pragma unroll
-                        for (uint32_t q = 0; q < kAhead; ++q) {
-                            const float *pi = part(min(i0 + q, parts - 1));
-                            f[q] = __ldcg(pi + RT * DH + n);
-                            z[q] = __ldcg(reinterpret_cast<const float2 *>(pi + n * DH + 2 * j));
-                        }
+                    for (uint32_t r = 0; r < kR; ++r) x[r] = y[r] = 0.f;
+                    for (uint32_t i0 = 0; i0 < parts; i0 += kP) {
+                        float f[kR][kP];
+                        float2 z[kR][kP];
 #pragma unroll
-                        for (uint32_t q = 0; q < kAhead; ++q) {
-                            if (i0 + q >= parts) continue;
-                            f[q] = f[q] == -INFINITY ? 0.f : fast_exp2(f[q] - mx);
-                            x = fmaf(z[q].x, f[q], x), y = fmaf(z[q].y, f[q], y);
-                        }
+                        for (uint32_t r = 0; r < kR; ++r)
+#pragma unroll
+                            for (uint32_t q = 0; q < kP; ++q) {
+                                const uint32_t n = n0 + r * kRowsPer;
+                                const float *pi = part(i0 + q);
+                                const bool in = n < nrows && i0 + q < parts;
+                                f[r][q] = in ? __ldcg(pi + RT * DH + n) : -INFINITY;
+                                z[r][q] = in ? __ldcg(reinterpret_cast<const float2 *>(pi + n * DH + 2 * j)) : make_float2(0.f, 0.f);
+                            }
+#pragma unroll
+                        for (uint32_t r = 0; r < kR; ++r)
+#pragma unroll
+                            for (uint32_t q = 0; q < kP; ++q) {
+                                const float mx = s_m[min(n0 + r * kRowsPer, nrows - 1)];
+                                const float g = f[r][q] == -INFINITY ? 0.f : fast_exp2(f[r][q] - mx);
+                                x[r] = fmaf(z[r][q].x, g, x[r]), y[r] = fmaf(z[r][q].y, g, y[r]);
+                            }
                     }
-                    write_out(n, d, x, y, ll);
+#pragma unroll
+                    for (uint32_t r = 0; r < kR; ++r) {
+                        const uint32_t n = n0 + r * kRowsPer;
+                        if (n < nrows) write_out(n, d, x[r], y[r], s_l[n]);
+                    }
                 }
             }
         }
@@ -1227,8 +1282,8 @@ constexpr size_t kCounterBytes = 16384;
 constexpr uint32_t kMaxSms = 160;         // the grid is cut there, so that the workspace is
 
 template <int DH, int NT, int NW, bool FP8>
-cudaError_t launch_rows(KvArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int sms, cudaStream_t st) {
-    constexpr uint32_t kPerSm = (NT == 1 ? 16 : 12) / NW;
+cudaError_t launch_rows(KvArgs &a, const CUtensorMap &mkv, int sms, cudaStream_t st) {
+    constexpr uint32_t kPerSm = (NT == 1 ? 16 : DH == 64 ? 12 : 8) / NW;
     static_assert(kMaxSms * kPerSm * 4 <= kCounterBytes &&
                       kCounterBytes + (size_t)2 * kPerSm * kMaxSms * 8 * NT * (DH + 2) * 4 <= SH_CUDA_KV8_WS_BYTES,
                   "workspace: a counter and two partial items per CTA");
@@ -1236,7 +1291,7 @@ cudaError_t launch_rows(KvArgs &a, const CUtensorMap &mk, const CUtensorMap &mv,
     auto kernel = k_attn_kv8_rows<DH, NT, NW, FP8>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSmem<DH, NT, NW>::kBytes);
     if (e != cudaSuccess) return e;
-    return sh::launch_pdl(kernel, dim3(sms * kPerSm), dim3(NW * 32), RowsSmem<DH, NT, NW>::kBytes, st, mk, mv, a);
+    return sh::launch_pdl(kernel, dim3(sms * kPerSm), dim3(NW * 32), RowsSmem<DH, NT, NW>::kBytes, st, mkv, a);
 }
 
 template <int DH, bool FP8>
@@ -1264,6 +1319,24 @@ bool kv_map(CUtensorMap *m, uint64_t base, const sh_cuda_kv8_t *c) {
     cuuint32_t box[3] = {c->dh, 16, 1};
     cuuint32_t estr[3] = {1, 1, 1};
     return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, (void *)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               c->dh == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// K and V codes as [2, pages, heads * page, dh] bytes, the lower array first (one of them where both are the same array):
+// boxes of 16 tokens of one page and head, of K and V at once; where pages allow it of the 32 tokens that a step takes.
+bool kv_pair_map(CUtensorMap *m, const sh_cuda_kv8_t *c, KvArgs &a) {
+    sh::PFN_encodeTiled enc = sh::encode_tiled();
+    if (!enc) return false;
+    const uint32_t step = 2048 / c->dh, rows = step < c->page ? step : c->page, arrays = c->k == c->v ? 1 : 2;
+    a.boxes = step / rows, a.box_bytes = arrays * rows * c->dh, a.box_step = a.boxes == 1 ? 16 * c->dh : 2048;
+    a.k_at = c->k <= c->v ? 0 : rows * c->dh, a.v_at = c->k < c->v ? rows * c->dh : 0;
+    const uint64_t lo = c->k < c->v ? c->k : c->v, hi = c->k < c->v ? c->v : c->k;
+    cuuint64_t dims[4] = {c->dh, (cuuint64_t)c->heads * c->page, c->pages, arrays};
+    cuuint64_t strides[3] = {c->dh, c->page_stride, arrays == 2 ? hi - lo : c->page_stride};
+    cuuint32_t box[4] = {c->dh, rows, 1, arrays};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, (void *)lo, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                c->dh == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -1308,22 +1381,23 @@ int sh_cuda_attention_kv8(uint64_t q, uint64_t o, const sh_cuda_kv8_t *c, uint64
     a.counters = (uint32_t *)ws, a.part = (float *)(ws + kCounterBytes), a.err = s.dev_err;
     const int sms = s.num_sms < (int)kMaxSms ? s.num_sms : (int)kMaxSms;
     const bool fp8 = c->fmt == SH_FP8, wide = (uint64_t)max_q * a.G > 8;
+    const bool tall = (uint64_t)max_q * a.G > 64;
     CUtensorMap mk, mv;
-    if (!kv_map(&mk, c->k, c) || !kv_map(&mv, c->v, c)) {
+    if (tall ? !kv_map(&mk, c->k, c) || !kv_map(&mv, c->v, c) : !kv_pair_map(&mk, c, a)) {
         sh::set_error(-1, "[sh_cuda_attention_kv8] no tensor map for the cache (page_stride=%llu)",
                       (unsigned long long)c->page_stride);
         return -1;
     }
     cudaError_t e;
     // Eight warps per CTA (two CTAs per SM) where items are fewer than SMs and many CTAs share one: half as many partial sums
-    // to join (131072 tokens of one request 56 us, 61 us with four). Four warps (four CTAs) where a CTA walks several items:
-    // the others go on while one ends an item (64 requests of up to 8192 tokens 109 us, 120 us with eight).
+    // to join (131072 tokens of one request 56 us, 63 us with four). Four warps (four CTAs) where a CTA walks several items:
+    // the others go on while one ends an item (64 requests of up to 8192 tokens 115 us, 123 us with eight).
     const bool few = (uint64_t)R * c->heads < (uint64_t)sms;
 #define SH_KV8(dh, nt, n) \
-    (fp8 ? launch_rows<dh, nt, n, true>(a, mk, mv, sms, s.stream) : launch_rows<dh, nt, n, false>(a, mk, mv, sms, s.stream))
-    // 64 rows are four tiles of the kernel above: 16 requests of 7 drafts (28 rows) 51 us there, 96 us here; 4 of 64 (256 rows)
-    // 107 us there, 68 us here.
-    if ((uint64_t)max_q * a.G > 64) {
+    (fp8 ? launch_rows<dh, nt, n, true>(a, mk, sms, s.stream) : launch_rows<dh, nt, n, false>(a, mk, sms, s.stream))
+    // 64 rows are four tiles of the kernel above: 16 requests of 7 drafts (28 rows) 77 us there, 128 us here; 4 of 64 (256 rows)
+    // 126 us there, 73 us here.
+    if (tall) {
         a.flip = scale < 0.f ? 0x80008000u : 0u;
         a.sl2 = fabsf(a.sl2);
         auto launch = c->dh == 64 ? (fp8 ? launch_tiles<64, true> : launch_tiles<64, false>)
