@@ -6,7 +6,7 @@
 // Bound by the weights' bytes (half a byte per element, read once), and close behind by the instructions that turn codes
 // into operands, so there are two forms of the inner product, both exact but for fp32 sums:
 //   fp16   code - zero is a small integer, exact in fp16: the 16-row operand of the matrix instruction (16 columns of W x
-//          16 k), 8 rows of X its columns, twice for up to 16 rows. 9 instructions turn a word into 8 operands (fp16
+//          16 k), 8 rows of X its columns, two or four times for more. 9 instructions turn a word into 8 operands (fp16
 //          patterns 1024 + c and 1024 + 16 c, then one subtraction or FMA).
 //   int8   for a single row and many columns: every finite fp16 value is an integer times 2^-24 below 2^41, i.e. six signed
 //          base-256 digits. The codes are int8 operands as they are (3 instructions per 8), the digits of X are six of the
@@ -316,7 +316,8 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
 
     auto bias_of = [&](uint32_t n) { return a.bias ? __half2float(a.bias[n]) : 0.f; };
     auto res_of = [&](uint32_t m, uint32_t n) { return a.res ? __half2float(a.res[(size_t)m * a.ldr + n]) : 0.f; };
-    // The output of a thread in each tile: at most one. A single row's sixteen go to the warps in turn.
+    // The outputs of a thread in each tile: one, or two sixteen rows apart. A single row's sixteen go to the warps in turn.
+    constexpr int kOut = NT > 2 ? 2 : 1;
     const uint32_t om = INT ? 0 : gt / kRows, orow = gt % kRows;
 
     const uint32_t swz = tile_row(g), w_at = smem_u32(ring) + swz * 128;
@@ -330,9 +331,14 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
         const int *xs = s_xs + (u0 - x0) * GU * kCols + 2 * c;
         // what the output adds is on its way while the products are taken
         const uint32_t on = tile * kRows + orow;
-        const bool mine = INT ? gw == (iter & 7) && lane < kRows : om < a.M;
-        const bool writes = mine && on < a.N && splits == 1;
-        const float bias = writes ? bias_of(on) : 0.f, res = writes ? res_of(om, on) : 0.f;
+        bool mine[kOut], writes[kOut];
+        float bias[kOut], res[kOut];
+#pragma unroll
+        for (int e = 0; e < kOut; ++e) {
+            mine[e] = INT ? gw == (iter & 7) && lane < kRows : om + 16 * e < a.M;
+            writes[e] = mine[e] && on < a.N && splits == 1;
+            bias[e] = writes[e] ? bias_of(on) : 0.f, res[e] = writes[e] ? res_of(om + 16 * e, on) : 0.f;
+        }
         const bool in_smem = staged(tile);
         const uint32_t sat = sc0 + turn * L.sc_bytes + 2 * (swz * groups + u0 * GU);
         const uint32_t zat = sc0 + turn * L.sc_bytes + 2 * kRows * groups + swz * groups + u0 * GU;
@@ -470,15 +476,19 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
         fence_proxy_async_smem();      // this tile's scales have been read: their buffer is copied into again
         group_sync();
         fetch_scales(tile + 2 * tile_step, turn);
-        float v = 0.f;
-        if (mine) {
 #pragma unroll
-            for (uint32_t w = 0; w < kGroupWarps; ++w) v += s_red[INT ? w * kRows + orow : (w * kCols + om) * kRows + orow];
-        }
-        if (splits > 1) {
-            if (mine) s_part[(iter * a.M + om) * kRows + orow] = v;
-        } else if (writes) {
-            finish(v, om, on, *s_flag, bias, res);
+        for (int e = 0; e < kOut; ++e) {
+            const uint32_t m = om + 16 * e;
+            float v = 0.f;
+            if (mine[e]) {
+#pragma unroll
+                for (uint32_t w = 0; w < kGroupWarps; ++w) v += s_red[INT ? w * kRows + orow : (w * kCols + m) * kRows + orow];
+            }
+            if (splits > 1) {
+                if (mine[e]) s_part[(iter * a.M + m) * kRows + orow] = v;
+            } else if (writes[e]) {
+                finish(v, m, on, *s_flag, bias[e], res[e]);
+            }
         }
         if (NT > 1) group_sync();
     }
@@ -527,7 +537,7 @@ bool w4_map(CUtensorMap *m, uint64_t codes, uint32_t N, uint32_t K, uint32_t ldw
 constexpr size_t kSmemMax = 227 * 1024, kMaxScales = 64 * 1024;
 
 template <int G, bool INT, int NT, int NG, int D>
-cudaError_t w4_try(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bool &fits) {
+cudaError_t w4_try(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bool &fits, uint32_t most = 8) {
     const uint32_t tiles = (a.N + 15) / 16, units = (a.K + kUnit - 1) / kUnit;
     uint32_t s = 1, room, iters;
     size_t smem;
@@ -539,7 +549,7 @@ cudaError_t w4_try(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bo
         iters = s > 1 ? (tiles + ctas * NG - 1) / (ctas * NG) : 0;      // sums kept for the cluster
         smem = w4_layout(NG, D, NT, kUnit / G, INT, a.zeros != nullptr, (units + s - 1) / s + 1, a.M,
                          a.staged ? a.K / G : 0, iters).bytes;
-        if (s == 8 || !((tiles * s * 2 <= (uint32_t)sms && units >= kGroupWarps * s * 2) || smem > kSmemMax)) break;
+        if (s == most || !((tiles * s * 2 <= (uint32_t)sms && units >= kGroupWarps * s * 2) || smem > kSmemMax)) break;
     }
     fits = smem <= kSmemMax;
     if (!fits) return cudaSuccess;
@@ -561,8 +571,8 @@ cudaError_t w4_try(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bo
     return cudaLaunchKernelEx(&cfg, kernel, mw, a, s, tiles, iters);
 }
 
-// Rows of X go in pieces of at most 16, and fewer when they do not fit beside each other. A second piece finds the weights
-// in L2 unless they are larger than that.
+// Rows of X go in one piece, or in pieces of at most 16 and fewer when they do not fit beside each other. A second piece finds
+// the weights in L2 unless they are larger than that.
 template <int G>
 cudaError_t w4_run(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bool &fits) {
     cudaError_t e = cudaSuccess;
@@ -571,6 +581,9 @@ cudaError_t w4_run(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bo
     if (a.M == 1 && tiles >= 3u * sms) e = w4_try<G, true, 1, 3, 2>(a, mw, sms, st, fits);
     if (!fits && e == cudaSuccess && a.M <= 8) e = w4_try<G, false, 1, 3, 2>(a, mw, sms, st, fits);
     if (e == cudaSuccess && a.M > 8 && a.M <= 16) e = w4_try<G, false, 2, 2, 2>(a, mw, sms, st, fits);
+    // all of up to 32 rows where X then needs no more than two parts of K (20 rows of 9000 x 2048 13.3 us, 16.3 in two pieces;
+    // with four parts 32 rows of 4096 x 4096 take 36 us, 19 in two pieces)
+    if (e == cudaSuccess && a.M > 16) e = w4_try<G, false, 4, 2, 2>(a, mw, sms, st, fits, 2);
     // long K: one group of warps, whose scales take less shared memory
     if (!fits && e == cudaSuccess && a.M == 1) e = w4_try<G, false, 1, 1, 3>(a, mw, sms, st, fits);
     if (fits || e != cudaSuccess || a.M == 1) return e;

@@ -571,6 +571,13 @@ def test_w4_single_row_of_many_columns(gpu_lib, group, zeros):
     _w4_case(gpu_lib, 1, 7200, 2048, group, zeros, L.EPI_BIAS, ldx=2055, offset=1)
 
 
+@pytest.mark.parametrize("M", [17, 25, 32])
+@pytest.mark.parametrize("K,N", [(256, 50), (1024, 600), (1568, 5000), (2048, 333), (4096, 1000)])
+def test_w4_up_to_32_rows(gpu_lib, M, K, N):
+    """In one pass and in pieces, K in one and in more parts, residual and bias of the upper rows."""
+    _w4_case(gpu_lib, M, N, K, 32, True, L.EPI_BIAS | L.EPI_RESIDUAL, ldx=K + 8, ldz=N + 3)
+
+
 @pytest.mark.parametrize("M", [1, 12])
 def test_w4_strides_and_odd_addresses(gpu_lib, M):
     for ldx, ldz, ldw, offset in ((520, 100, 256, 0), (513, 97, 272, 0), (512, 96, 1024, 1)):
