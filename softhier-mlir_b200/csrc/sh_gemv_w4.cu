@@ -23,6 +23,8 @@
 // instruction is free when both operands agree. A tile's scales and zero points come as rows of 16 bytes, one tile
 // ahead. When the columns alone do not fill the GPU, the CTAs of a cluster share K. All partial sums meet in shared
 // memory in a fixed order.
+#include <atomic>
+
 #include "sh_internal.cuh"
 
 namespace {
@@ -536,6 +538,29 @@ bool w4_map(CUtensorMap *m, uint64_t codes, uint32_t N, uint32_t K, uint32_t ldw
 
 constexpr size_t kSmemMax = 227 * 1024, kMaxScales = 64 * 1024;
 
+// Clusters of s CTAs (one per SM) that run at once: the GPU's SMs come in groups that a cluster does not cross, so there are
+// fewer than num_sms / s of them (33 of 4, not 37), and one more would be a second wave. A property of the device, asked once.
+template <typename K>
+uint32_t w4_clusters(K kernel, uint32_t threads, uint32_t s, uint32_t sms) {
+    if (s == 1) return sms;
+    static std::atomic<uint32_t> known[sh::kMaxDevices][9];      // s is 2, 4 or 8
+    std::atomic<uint32_t> &k = known[sh::state().device % sh::kMaxDevices][s];
+    uint32_t n = k.load(std::memory_order_relaxed);
+    if (n == 0) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(1, s), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = kSmemMax;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 1, attr[0].val.clusterDim.y = s, attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr, cfg.numAttrs = 1;
+        int got = 0;
+        n = sms / s;
+        if (cudaOccupancyMaxActiveClusters(&got, kernel, &cfg) == cudaSuccess && got > 0 && (uint32_t)got < n) n = (uint32_t)got;
+        k.store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
 template <int G, bool INT, int NT, int NG, int D>
 cudaError_t w4_try(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bool &fits, uint32_t most = 8) {
     const uint32_t tiles = (a.N + 15) / 16, units = (a.K + kUnit - 1) / kUnit;
@@ -543,8 +568,11 @@ cudaError_t w4_try(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bo
     size_t smem;
     // K parts over a cluster while the columns alone leave SMs idle and every warp keeps a step, or until X fits
     a.staged = (((uint64_t)a.scales | (uint64_t)a.zeros) & 15) == 0 && a.K % kUnit == 0 && a.K / G * 96 <= kMaxScales / NG;
+    auto kernel = a.zeros ? k_gemv_w4<G, INT, NT, NG, D, true> : k_gemv_w4<G, INT, NT, NG, D, false>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax);
+    if (e != cudaSuccess) return e;
     for (;; s *= 2) {
-        room = (uint32_t)sms / s;
+        room = w4_clusters(kernel, NG * kGroupThreads, s, (uint32_t)sms);
         const uint32_t ctas = tiles < room ? tiles : room;
         iters = s > 1 ? (tiles + ctas * NG - 1) / (ctas * NG) : 0;      // sums kept for the cluster
         smem = w4_layout(NG, D, NT, kUnit / G, INT, a.zeros != nullptr, (units + s - 1) / s + 1, a.M,
@@ -553,9 +581,6 @@ cudaError_t w4_try(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bo
     }
     fits = smem <= kSmemMax;
     if (!fits) return cudaSuccess;
-    auto kernel = a.zeros ? k_gemv_w4<G, INT, NT, NG, D, true> : k_gemv_w4<G, INT, NT, NG, D, false>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax);
-    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(tiles < room ? tiles : room, s);
     cfg.blockDim = dim3(NG * kGroupThreads);
@@ -582,7 +607,7 @@ cudaError_t w4_run(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bo
     if (!fits && e == cudaSuccess && a.M <= 8) e = w4_try<G, false, 1, 3, 2>(a, mw, sms, st, fits);
     if (e == cudaSuccess && a.M > 8 && a.M <= 16) e = w4_try<G, false, 2, 2, 2>(a, mw, sms, st, fits);
     // all of up to 32 rows where X then needs no more than two parts of K (20 rows of 9000 x 2048 13.3 us, 16.3 in two pieces;
-    // with four parts 32 rows of 4096 x 4096 take 36 us, 19 in two pieces)
+    // with four parts 32 rows of 4096 x 4096 take 20.4 us, 19.3 in two pieces)
     if (e == cudaSuccess && a.M > 16) e = w4_try<G, false, 4, 2, 2>(a, mw, sms, st, fits, 2);
     // long K: one group of warps, whose scales take less shared memory
     if (!fits && e == cudaSuccess && a.M == 1) e = w4_try<G, false, 1, 1, 3>(a, mw, sms, st, fits);
