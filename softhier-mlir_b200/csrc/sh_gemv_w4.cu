@@ -13,7 +13,7 @@
 //          instruction's eight columns, of which a single row would leave seven empty, and the int32 sums of a group are
 //          exact. The zero point enters as -zero sum(digits). A 16 x 128 step takes 4 matrix instructions and 24 others, not
 //          8 and 72, but the digits take longer to lay out, so that it pays from about three tiles per SM on
-//          (49152 x 4096: 23.3 us, 30.3 us in fp16; 4096 x 4096: 5.6 us, 4.8 us in fp16).
+//          (49152 x 4096: 23.9 us, 30 us in fp16; 4096 x 4096: 5.6 us, 4.8 us in fp16).
 //          Infinities and NaN have no digits; outputs of such a row get those terms one by one.
 //
 // One CTA per SM: X is laid out in shared memory once, then groups of 8 warps walk tiles of 16 columns of W, each warp an
@@ -569,8 +569,13 @@ cudaError_t w4_try(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bo
     // K parts over a cluster while the columns alone leave SMs idle and every warp keeps a step, or until X fits
     a.staged = (((uint64_t)a.scales | (uint64_t)a.zeros) & 15) == 0 && a.K % kUnit == 0 && a.K / G * 96 <= kMaxScales / NG;
     auto kernel = a.zeros ? k_gemv_w4<G, INT, NT, NG, D, true> : k_gemv_w4<G, INT, NT, NG, D, false>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax);
-    if (e != cudaSuccess) return e;
+    static bool done[2][sh::kMaxDevices] = {};
+    bool &ready = done[a.zeros != nullptr][sh::current_device() % sh::kMaxDevices];
+    if (!ready) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax);
+        if (e != cudaSuccess) return e;
+        ready = true;
+    }
     for (;; s *= 2) {
         room = w4_clusters(kernel, NG * kGroupThreads, s, (uint32_t)sms);
         const uint32_t ctas = tiles < room ? tiles : room;
