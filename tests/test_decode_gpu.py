@@ -509,6 +509,31 @@ def test_attention_infinite_and_nan_queries_stay_in_their_rows(gpu_lib, nq):
         assert np.array_equal(bits[rest], good[rest])
 
 
+@pytest.mark.parametrize("max_q", [1, 12, 80])
+def test_attention_idle_requests_and_fewer_rows_than_q_start(gpu_lib, max_q):
+    """Nothing is written where no request has a row, nor past T when q_start goes further."""
+    rt = gpu_lib
+    pool = Pool(8, 2, 32, 64, "int8", 4)
+    q = torch.randn((170, 256), device=DEV, generator=torch.Generator(DEV).manual_seed(2)).half()
+    table, lens = _i32([[0, 1, 2, 3], [4, 5, 6, 7]]), _i32([100, 128])
+    ws = torch.zeros(L.KV8_WS_BYTES, dtype=torch.uint8, device=DEV)
+
+    def run(starts, T):
+        o, s = torch.full_like(q, 7.0), _i32(starts)
+        assert rt.lib.sh_cuda_attention_kv8(_p(q), _p(o), pool.handle, _p(table), 4, _p(lens), _p(s), 2, T, max_q, 4, 256, 256,
+                                            0.125, _p(ws), ws.numel()) == 0
+        rt.check()
+        return _np(o)
+    assert (run([5, 5, 5], 170) == 7).all()
+    whole, cut = run([0, 80, 160], 170), run([0, 80, 160], 111)
+    # both round the output and the weights by half a step (2^-11 of at most the largest value each); sums in fp32 beside that
+    vmax = np.abs(D.decode(pool.codes[1], "int8") * pool.scales[1][:, :, None, None]).max()
+    assert np.abs(cut[:111].astype(np.float64) - whole[:111]).max() <= 2 * 2.5 * 2.0 ** -11 * vmax
+    assert (cut[111:] == 7).all() and (whole[160:] == 7).all() and (whole[:160] != 7).any(1).all()
+    late = run([3, 83, 163], 170)
+    assert (late[:3] == 7).all() and (late[163:] == 7).all() and (late[3:163] != 7).any(1).all()
+
+
 # ---- 4-bit weights -------------------------------------------------------------------------------------------------------
 def _w4_case(rt, M, N, K, group, zeros, epi=0, ldx=None, ldz=None, ldw=None, offset=0, seed=0):
     rng = np.random.default_rng(seed + M + N + K)
