@@ -1,4 +1,4 @@
-"""64-bit CPU statement of the decode-step operators (test infrastructure only: the checker, never the product path).
+"""64-bit CPU statement of the decode-step operators (test infrastructure only, never the product path).
 
 Semantics: include/sh_ops_cuda.h, "decoding: paged 8-bit K / V cache and 4-bit weights". Written as plain loops over
 requests, pages and groups.
