@@ -721,8 +721,8 @@ struct TilesSmem {
     static constexpr uint32_t kQ = 0, kK = kQ + 2 * kTile, kV = kK + 2 * kTile, kRing = kV + kTile;   // K twice
     static constexpr uint32_t kInfo = kRing + kTlStages * 2 * kCodes;  // [stages][8] {ks, vs, usable}
     static constexpr uint32_t kGroup = kInfo + kTlStages * 128;        // [4][8] {ks scale log2 e, log2 vs, 1 / vs}
-    static constexpr uint32_t kRowMax = kGroup + 512;                  // [2 tiles][2][128] bf16
-    static constexpr uint32_t kBars = kRowMax + 1024, kMisc = kBars + 24 * 8, kBytes = kMisc + 320;
+    static constexpr uint32_t kRowMax = kGroup + 512;                  // [2 tiles][2][128]
+    static constexpr uint32_t kBars = kRowMax + 2048, kMisc = kBars + 20 * 8, kBytes = kMisc + 64;
     static_assert(kBytes <= 227 * 1024, "shared memory");
 };
 
@@ -780,12 +780,13 @@ __global__ void __launch_bounds__(kTlThreads, 1)
     uint64_t *k_full = bars + 4, *k_empty = bars + 18, *v_full = bars + 6, *v_empty = bars + 7;   // K: two each
     uint64_t *q_full = bars + 8, *s_full = bars + 10, *p_full = bars + 12, *o_full = bars + 14, *mdone = bars + 16;
     struct Misc {
-        u64 part[kTlThreads / 32];
         TileCursor first;
         uint32_t flag, tmem;
         int abort;
     };
+    static_assert(sizeof(Misc) <= SM::kBytes - SM::kMisc, "shared memory");
     Misc &mi = *reinterpret_cast<Misc *>(sm + SM::kMisc);
+    u64 *warp_units = reinterpret_cast<u64 *>(sm + SM::kRowMax);      // read before the first maximum is written
     volatile int *abort = &mi.abort;
     const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const uint32_t page1 = (1u << a.page_shift) - 1;
@@ -836,12 +837,12 @@ __global__ void __launch_bounds__(kTlThreads, 1)
         const u64 x = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= (uint32_t)o) incl += x;
     }
-    if (lane == 31) mi.part[warp] = incl;
+    if (lane == 31) warp_units[warp] = incl;
     __syncthreads();
     u64 total = 0;
     for (uint32_t w = 0; w < kTlThreads / 32; ++w) {
-        if (w < warp) incl += mi.part[w];
-        total += mi.part[w];
+        if (w < warp) incl += warp_units[w];
+        total += warp_units[w];
     }
     const u64 per = (total + gridDim.x - 1) / gridDim.x, begin = per * blockIdx.x, end = min(total, begin + per);
     if (begin < end && begin >= incl - sum && begin < incl) {
@@ -1035,8 +1036,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
         constexpr uint32_t kHalfKeys = kTlKeys / 2, kHalfCols = DH / 2;
         const uint32_t lane_base = tmem + (quarter * 32u << 16);
         const uint32_t s_addr = lane_base + kTmS + t2 * kTlKeys, o_addr = lane_base + kTmO + t2 * DH + half * kHalfCols;
-        // [2][128] of the tile: the halves' maxima, as bf16 towards +infinity, so that both go on with the same value
-        uint16_t *row_max = reinterpret_cast<uint16_t *>(sm + SM::kRowMax) + t2 * 256 + row;
+        float *row_max = reinterpret_cast<float *>(sm + SM::kRowMax) + t2 * 256 + row;            // [2][128] of the tile: the halves' maxima
         float *row_sum = reinterpret_cast<float *>(sm + SM::kQ + t2 * SM::kTile) + row;           // over Q at an item's end
         uint32_t n = 0, sn = 0, on = 0;      // blocks of the run, blocks of this tile, items of this tile
         TileCursor k = k0;
@@ -1113,10 +1113,9 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                     const float a3 = max3(x[9], x[10], x[11]), a4 = max3(x[12], x[13], x[14]);
                     mb = fmaxf(mb, fmaf(max3(max3(a0, a1, a2), fmaxf(a3, a4), x[15]), gr.x, gr.y));
                 }
-                const uint32_t up = (__float_as_uint(mb) + (mb > 0.f ? 0xFFFFu : 0u)) >> 16;
-                row_max[half * 128] = (uint16_t)up;
+                row_max[half * 128] = mb;
                 tile_sync();      // both halves' maxima are there, and both hold their scores: P may go over S
-                mb = fmaxf(__uint_as_float(up << 16), __uint_as_float((uint32_t)row_max[(half ^ 1) * 128] << 16));
+                mb = fmaxf(mb, row_max[(half ^ 1) * 128]);
                 // the maximum only moves when a weight would pass 2^8 (exact room in fp16); O is rescaled then
                 float alpha = 1.f;
                 const bool raise = mb > m + 8.f;

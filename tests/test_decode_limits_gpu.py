@@ -1,0 +1,72 @@
+"""The decode-step operators at the edges of what their header allows."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import decode as D
+from softhier_cuda import lib as L
+from test_decode_gpu import DEV, Pool, _i32, _np, _p
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- softmax exponents far from zero -------------------------------------------------------------------------------------
+def _offset_case(rt, fmt, dh, nq, big, max_q, seed=1):
+    """The scores of a row share a large offset: column 0 of every key is 96, of every row +-`big`; the other columns are small
+    whole numbers. All sums are whole numbers below 2^24 and the scales powers of two, so the scores themselves are exact.
+    -> outputs, oracle's outputs, tolerance."""
+    rng = np.random.default_rng(seed)
+    H, heads, page = 4, 2, 32
+    lens = np.array([300, 47 + nq])
+    blocks = -(-lens // page)
+    pages = int(blocks.sum())
+    pool = Pool(pages, heads, page, dh, fmt, seed)
+    k = rng.integers(-3, 4, pool.shape).astype(np.float64)
+    k[..., 0] = 96
+    pool.codes[0] = D.encode(k, fmt)
+    pool.scales[0] = np.full((pages, heads), 2.0 ** -5, np.float32)
+    pool.scales[1] = np.full((pages, heads), 2.0 ** -6, np.float32)
+    raw = np.stack(pool.codes)
+    pool.raw.copy_(torch.from_numpy(raw.reshape(-1)))
+    for i in range(2):
+        pool.dev_scales[i].copy_(torch.from_numpy(pool.scales[i]))
+    table = np.zeros((2, int(blocks.max())), np.int64)
+    table[0, :blocks[0]], table[1, :blocks[1]] = np.arange(blocks[0]), blocks[0] + np.arange(blocks[1])
+    q_start = np.array([0, nq, 2 * nq])
+    T = 2 * nq
+    q = rng.integers(-2, 3, (T, H, dh)).astype(np.float16)
+    q[:, :, 0] = big * np.where((np.arange(T)[:, None] + np.arange(H)) % 2, -1, 1)
+    q = q.reshape(T, H * dh)
+    scale = 2.0 ** (2 if dh == 64 else 1)
+    dq, do, ws = torch.from_numpy(q).to(DEV), torch.zeros((T, H * dh), dtype=torch.float16, device=DEV), \
+        torch.zeros(L.KV8_WS_BYTES, dtype=torch.uint8, device=DEV)
+    d_table, d_lens, d_start = _i32(table), _i32(lens), _i32(q_start)
+    assert rt.lib.sh_cuda_attention_kv8(_p(dq), _p(do), pool.handle, _p(d_table), table.shape[1], _p(d_lens), _p(d_start), 2, T,
+                                        max_q, H, H * dh, H * dh, scale, _p(ws), ws.numel()) == 0
+    rt.check()
+    want, mean_abs, _, _ = D.attention_kv8(q, *pool.codes, *pool.scales, table, lens, q_start, H, scale, fmt)
+    # Exponents of two of up to E = scale log2(e) (96 big + 2 * 3 * dh) 2^-5, each rounded twice on its way (its multiply-add; the
+    # maximum that is taken off), in numerator and denominator: 4 half steps of 2^-24 E, times ln 2 < 1; 2^-21 for exp2 and
+    # the products by the factors of a moved maximum; a half step of fp16 for the weights (2^-25 of the largest for those
+    # below the normal range) and one for the output; fp32 sums over the keys.
+    n = float(lens.max())
+    E = scale * 1.4427 * (96 * big + 6 * dh) / 32 + 6
+    vmax = np.abs(D.decode(pool.codes[1], fmt) * pool.scales[1][:, :, None, None]).max()
+    tol = 2.0 ** -11 * np.abs(want) + 2.0 ** -25 + (2.0 ** -11 + 4 * 2.0 ** -24 * E + 2.0 ** -21 + 2 * n * 2.0 ** -24) * 1.01 * mean_abs \
+        + n * 2.0 ** -25 * vmax
+    return _np(do).astype(np.float64), want, tol
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("nq,max_q", [(1, 1), (30, 30), (80, 80), (1, 80)])
+@pytest.mark.parametrize("big", [16, 180, 300, 2047])
+def test_attention_depends_on_score_differences_only(gpu_lib, fmt, dh, nq, max_q, big):
+    """Exponents of up to about +-280, 3100, 5200 and 35000 (half of that at dh = 128): the row's maximum is taken off whole,
+    however large it is."""
+    got, want, tol = _offset_case(gpu_lib, fmt, dh, nq, big, max_q)
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:4], got[bad][:4], want[bad][:4])
+    assert (np.abs(got).max(1) > 0).all()
