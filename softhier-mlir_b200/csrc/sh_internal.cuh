@@ -14,6 +14,7 @@
 #include <stdio.h>
 #include <stdlib.h>
 
+#include <atomic>
 #include <utility>
 
 #include "sh_ops.h"
@@ -104,6 +105,17 @@ cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t s
     return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
+// Lets Kernel have up to `bytes` of dynamic shared memory (the same at every call), once per device. Without it 48 KiB hold
+// its static and its dynamic part together. Host threads may call it at the same time: the attribute is then set twice.
+template <auto Kernel>
+cudaError_t allow_smem(size_t bytes) {
+    static std::atomic<bool> done[kMaxDevices];
+    std::atomic<bool> &d = done[current_device() % kMaxDevices];
+    if (d.load(std::memory_order_acquire)) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) d.store(true, std::memory_order_release);
+    return e;
+}
 
 }  // namespace sh
 

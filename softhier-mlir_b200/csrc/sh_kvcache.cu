@@ -481,8 +481,7 @@ int sh_cuda_kv_tables(uint64_t lens, uint64_t add, uint32_t R, uint32_t page, ui
     const uint32_t grid = want < 1 ? 1 : want < cap ? (uint32_t)want : cap;
     const size_t smem = (size_t)R * 16;
     auto kernel = per == 4 ? k_kv_tables<4> : k_kv_tables<1>;
-    if (smem > 48 * 1024 &&
-        !sh::cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kTabMaxR * 16)),
+    if (!sh::cuda_ok(per == 4 ? sh::allow_smem<k_kv_tables<4>>(kTabMaxR * 16) : sh::allow_smem<k_kv_tables<1>>(kTabMaxR * 16),
                      "sh_cuda_kv_tables"))
         return -1;
     return sh::cuda_ok(sh::launch_pdl(kernel, dim3(grid), dim3(kTabThreads), smem, s.stream, a), "sh_cuda_kv_tables") ? 0 : -1;

@@ -1,6 +1,10 @@
 """The decode-step operators at the edges of what their header allows."""
 from __future__ import annotations
 
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -70,3 +74,12 @@ def test_attention_depends_on_score_differences_only(gpu_lib, fmt, dh, nq, max_q
     bad = ~(np.abs(got - want) <= tol)
     assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:4], got[bad][:4], want[bad][:4])
     assert (np.abs(got).max(1) > 0).all()
+
+
+# ---- tables: shared memory around 48 KiB ---------------------------------------------------------------------------------
+@pytest.mark.parametrize("many_rows", [False, True])
+def test_tables_of_sizes_around_48_kib_of_shared_memory(many_rows):
+    """In a process of its own, as the border depends on what was called before."""
+    worker = Path(__file__).resolve().parent / "tables_worker.py"
+    r = subprocess.run([sys.executable, str(worker), "many" if many_rows else "few"], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "OK" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
