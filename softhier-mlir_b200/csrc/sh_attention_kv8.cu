@@ -36,16 +36,19 @@ struct KvArgs {
 // A request as the kernels see it: lengths that no index leaves the arrays with, whatever the device arrays hold.
 struct ReqView {
     uint32_t qs, nq, ctx;
-    int base;             // tokens before its first new row (< 0: the first rows have none)
+    int base;             // tokens before its first new row (< 0: the first rows have none), at most ctx
 };
 __device__ __forceinline__ ReqView req_view(const KvArgs &a, uint32_t r) {
     ReqView v;
-    const int s = a.q_start[r], e = a.q_start[r + 1], len = a.lens[r];
+    const int s = a.q_start[r], e = a.q_start[r + 1], len = max(a.lens[r], 0);
     const int s0 = min(max(s, 0), (int)a.T), e0 = min(max(e, s0), (int)a.T);
     v.qs = (uint32_t)s0;
     v.nq = (uint32_t)(e0 - s0);
-    v.ctx = min((uint32_t)max(len, 0), a.ld_table << a.page_shift);
-    v.base = (int)v.ctx - max(e - s, 0) + (s0 - s);
+    v.ctx = min((uint32_t)len, a.ld_table << a.page_shift);
+    // of the length as it is: a row's limit counts tokens past the table, which are then left out. Below -nq and above ctx
+    // nothing changes.
+    const long long base = (long long)len - max((long long)e - s, 0ll) + (s0 - (long long)s);
+    v.base = (int)min(max(base, -(long long)v.nq), (long long)v.ctx);
     return v;
 }
 

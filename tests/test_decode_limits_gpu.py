@@ -11,7 +11,7 @@ import torch
 
 from oracle import decode as D
 from softhier_cuda import lib as L
-from test_decode_gpu import DEV, Pool, _i32, _np, _p
+from test_decode_gpu import DEV, Pool, _attn_tol, _i32, _np, _p
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +83,38 @@ def test_tables_of_sizes_around_48_kib_of_shared_memory(many_rows):
     worker = Path(__file__).resolve().parent / "tables_worker.py"
     r = subprocess.run([sys.executable, str(worker), "many" if many_rows else "few"], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "OK" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
+
+
+# ---- lengths past the table -----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("nq", [1, 3, 12, 80])
+@pytest.mark.parametrize("over", [1, 2, 40, 1000, 2 ** 31 - 1 - 64])
+def test_attention_of_a_length_past_the_table(gpu_lib, nq, over):
+    """Row i attends the tokens j <= lens - n + i that the table has: of a length `over` past it the last `over` rows attend all of
+    them, and the rows before as in a request of n - over rows that ends with the table."""
+    rt = gpu_lib
+    page, heads, dh, H, cap = 16, 2, 64, 4, 64
+    pool = Pool(8, heads, page, dh, "int8", 4)
+    table = np.array([[0, 1, 2, 3], [4, 5, 6, 7]])
+    rng = np.random.default_rng(nq)
+    q = rng.standard_normal((2 * nq, H * dh)).astype(np.float16)
+    dq, do = torch.from_numpy(q).to(DEV), torch.zeros((2 * nq, H * dh), dtype=torch.float16, device=DEV)
+    d = _i32(table), _i32([cap + over, 50]), _i32([0, nq, 2 * nq])
+    ws = torch.zeros(L.KV8_WS_BYTES, dtype=torch.uint8, device=DEV)
+    assert rt.lib.sh_cuda_attention_kv8(_p(dq), _p(do), pool.handle, _p(d[0]), 4, _p(d[1]), _p(d[2]), 2, 2 * nq, nq, H, H * dh, H * dh,
+                                        0.125, _p(ws), ws.numel()) == 0
+    assert rt.lib.sh_cuda_device_error() == 2
+    early = max(nq - over, 0)
+    starts, lens = [0], []
+    if early:
+        starts, lens = [0, early], [cap]
+    for _ in range(early, nq):
+        starts.append(starts[-1] + 1)
+        lens.append(cap)
+    starts.append(2 * nq)
+    lens.append(50)
+    rows = np.concatenate([np.repeat(table[:1], len(lens) - 1, 0), table[1:]])
+    want, mean_abs, big, keys = D.attention_kv8(q, *pool.codes, *pool.scales, rows, lens, starts, H, 0.125, "int8")
+    vmax = np.abs(D.decode(pool.codes[1], "int8") * pool.scales[1][:, :, None, None]).max()
+    err = np.abs(_np(do).astype(np.float64) - want)
+    tol = _attn_tol(want, mean_abs, big, keys, H, dh, vmax)
+    assert (err <= tol).all(), np.argwhere(err > tol)[:4]
