@@ -180,8 +180,8 @@ int sh_cuda_kv8_append(const sh_cuda_kv8_t *cache, uint64_t k, uint64_t v, uint3
  * served, in any mixture. q holds T rows; max_q, the most rows of one request, only picks the kernel (a wrong value
  * costs time). ws: ws_bytes >= SH_CUDA_KV8_WS_BYTES of device memory, 16-byte aligned, zeroed once before its first use,
  * for the calls of one stream at a time (a graph that may run beside other calls has its own). A table entry outside the
- * cache, or a length past ld_table * page, raises the device error word (2) and those tokens are left out. Returns 0,
- * -1, or -3 for fmt. */
+ * cache, or a length past ld_table * page, raises the device error word (2) and those tokens are left out. T * H < 2^31 and
+ * T + ld_table * page <= 2^31 - 2^14. Returns 0, -1, or -3 for fmt. */
 #define SH_CUDA_KV8_WS_BYTES (48u << 20)
 int sh_cuda_attention_kv8(uint64_t q, uint64_t o, const sh_cuda_kv8_t *cache, uint64_t table, uint32_t ld_table,
                           uint64_t lens, uint64_t q_start, uint32_t R, uint32_t T, uint32_t max_q, uint32_t H,

@@ -1282,6 +1282,9 @@ __global__ void __launch_bounds__(kTlThreads, 1)
 
 constexpr size_t kCounterBytes = 16384;
 constexpr uint32_t kMaxSms = 160;         // the grid is cut there, so that the workspace is
+// Token numbers are int in the kernels, and they run ahead of a request's last token by up to 32 units of 256 when page ids are
+// read, by a block of a tile, and by its new rows in a row's limit.
+constexpr uint64_t kMaxTokens = (1ull << 31) - (1u << 14);
 
 template <int DH, int NT, int NW, bool FP8>
 cudaError_t launch_rows(KvArgs &a, const CUtensorMap &mkv, int sms, cudaStream_t st) {
@@ -1364,10 +1367,11 @@ int sh_cuda_attention_kv8(uint64_t q, uint64_t o, const sh_cuda_kv8_t *c, uint64
     const int bad = sh::kv8_check(c, "sh_cuda_attention_kv8");
     if (bad) return bad;
     if (H == 0 || H % c->heads || (uint64_t)H * c->dh > ldq || (uint64_t)H * c->dh > ldo ||
-        (uint64_t)T * H >= (1ull << 31) || ld_table == 0 || ld_table >= (1u << 31) / c->page || !(fabsf(scale) < INFINITY)) {
-        sh::set_error(-1, "[sh_cuda_attention_kv8] need H a multiple of the cache's %u heads, ldq, ldo >= H dh, T H and "
-                      "ld_table page < 2^31, a finite scale (H=%u ldq=%u ldo=%u T=%u ld_table=%u)", c->heads, H, ldq, ldo,
-                      T, ld_table);
+        (uint64_t)T * H >= (1ull << 31) || ld_table == 0 || T + (uint64_t)ld_table * c->page > kMaxTokens ||
+        !(fabsf(scale) < INFINITY)) {
+        sh::set_error(-1, "[sh_cuda_attention_kv8] need H a multiple of the cache's %u heads, ldq, ldo >= H dh, T H < 2^31, "
+                      "T + ld_table page <= 2^31 - 2^14, a finite scale (H=%u ldq=%u ldo=%u T=%u ld_table=%u)", c->heads, H,
+                      ldq, ldo, T, ld_table);
         return -1;
     }
     if (!ws || !sh::aligned16(ws) || ws_bytes < SH_CUDA_KV8_WS_BYTES) {

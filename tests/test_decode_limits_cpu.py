@@ -1,0 +1,21 @@
+"""Limits of the decode-step operators that need no GPU: what is refused before any CUDA call, and what their sources must hold."""
+from __future__ import annotations
+
+import pytest
+
+from softhier_cuda import lib as L
+from test_decode_cpu import _attn, _cache, lib  # noqa: F401  (lib: the fixture)
+
+
+@pytest.mark.parametrize("page", [16, 128])
+def test_attention_refuses_tables_whose_tokens_pass_31_bits(lib, capfd, page):      # noqa: F811
+    """Token numbers run ahead of a request's last one, so a table has to end 2^14 tokens before 2^31."""
+    lib.sh_cuda_last_error()
+    most = ((1 << 31) - (1 << 14)) // page
+    cache = _cache(page=page, page_stride=4 * page * 64)
+    for ld_table, T in ((most, 1), (most + 1, 0), (most - 8, 1 << 27), ((1 << 31) // page - 1, 0), ((1 << 32) // page, 0)):
+        assert _attn(lib, cache, ld_table=ld_table, T=T, H=4, ldq=256, ldo=256) == -1, (ld_table, T)
+        assert "need H a multiple" in capfd.readouterr().out
+    assert _attn(lib, cache, ld_table=most, T=0) == 0
+    lib.sh_cuda_last_error()
+    capfd.readouterr()
