@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : DH == 64 ? 12 : 8) / 
             scales[1][f] = make_float2(0.f, -1.f);
             if ((uint32_t)id[f] < a.pages) {
                 const size_t at = (size_t)id[f] * a.heads + p.kvh;
-                scales[1][f] = make_float2(__ldg(a.ks + at), __ldg(a.vs + at));
+                scales[1][f] = make_float2(a.ks[at], a.vs[at]);
             } else if ((int)(tok + f * 16) < p.lim_hi && lane == 0) {
                 atomicCAS(a.err, 0, (int)sh::kErrBadArgs);
             }

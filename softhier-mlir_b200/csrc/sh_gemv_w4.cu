@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(NG * kGroupThreads, 1)
             if (p < per_row * a.M && at < a.K) {
                 const __half *xp = a.x + (size_t)m * a.ldx + at;
                 if (a.vec) {
-                    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(xp));
+                    const uint4 v = __ldcg(reinterpret_cast<const uint4 *>(xp));      // once per CTA: past the L1
                     x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
                 } else {
 #pragma unroll

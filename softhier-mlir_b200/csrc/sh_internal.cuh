@@ -181,7 +181,8 @@ __device__ __forceinline__ uint32_t atom_add_acq_rel_gpu(uint32_t *p, uint32_t v
 
 // Programmatic dependent launch: a kernel launched with cudaLaunchAttributeProgrammaticStreamSerialization may
 // start while its stream predecessor still runs; pdl_wait() blocks until that predecessor has completed and its
-// memory is visible, so everything before it must touch no memory a predecessor writes or reads.
+// memory is visible, so everything before it must touch no memory a predecessor writes or reads. What a predecessor writes is
+// read with plain loads (or __ldcg): __ldg promises data that nobody writes while the kernel lives, and it lives before the wait.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -260,7 +260,7 @@ __device__ __forceinline__ float decode(uint32_t c) {
 template <bool VEC>
 __device__ __forceinline__ void raw8(uint32_t (&w)[4], const __half *p) {
     if (VEC) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
+        const uint4 v = __ldcg(reinterpret_cast<const uint4 *>(p));
         w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
     } else {
 #pragma unroll

@@ -1,10 +1,14 @@
 """Limits of the decode-step operators that need no GPU: what is refused before any CUDA call, and what their sources must hold."""
 from __future__ import annotations
 
+from pathlib import Path
+
 import pytest
 
 from softhier_cuda import lib as L
 from test_decode_cpu import _attn, _cache, lib  # noqa: F401  (lib: the fixture)
+
+CSRC = Path(__file__).resolve().parents[1] / "softhier-mlir_b200" / "csrc"
 
 
 @pytest.mark.parametrize("page", [16, 128])
@@ -19,3 +23,11 @@ def test_attention_refuses_tables_whose_tokens_pass_31_bits(lib, capfd, page):  
     assert _attn(lib, cache, ld_table=most, T=0) == 0
     lib.sh_cuda_last_error()
     capfd.readouterr()
+
+
+@pytest.mark.parametrize("name", ["sh_kvcache.cu", "sh_attention_kv8.cu", "sh_gemv_w4.cu"])
+def test_decode_kernels_read_what_predecessors_write_with_plain_loads(name):
+    """Each operator of a step reads what the one before it wrote, and may be launched while that one still runs: loads that
+    promise constant data for the kernel's whole life have no place there."""
+    src = (CSRC / name).read_text()
+    assert "__ldg(" not in src and "ld.global.nc" not in src and "__restrict__" not in src
