@@ -891,11 +891,13 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                 if (n >= kTlStages) mbar_wait(c_empty + st, ph ^ 1u, abort, a.err);
                 uint64_t *bar = c_full + st;
                 const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, ok));
+                float *info = reinterpret_cast<float *>(sm + SM::kInfo + (st * 8 + lane) * 16);
+                // the lanes' own stores come before lane 0's arrival, which releases them (theirs below only count copies)
+                if (lane < 8) info[2] = ok;
+                __syncwarp();
                 if (lane == 0) mbar_arrive_expect_tx(bar, boxes * 2 * SM::kBox);
                 __syncwarp();
                 if (lane < 8) {
-                    float *info = reinterpret_cast<float *>(sm + SM::kInfo + (st * 8 + lane) * 16);
-                    info[2] = ok;
                     if (ok) {
                         uint8_t *dst = sm + SM::kRing + st * 2 * SM::kCodes + lane * SM::kBox;
                         tma_load_3d(dst, &mk, bar, 0, row, page);

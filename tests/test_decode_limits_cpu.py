@@ -31,3 +31,12 @@ def test_decode_kernels_read_what_predecessors_write_with_plain_loads(name):
     promise constant data for the kernel's whole life have no place there."""
     src = (CSRC / name).read_text()
     assert "__ldg(" not in src and "ld.global.nc" not in src and "__restrict__" not in src
+
+
+def test_the_copy_warp_stores_a_stages_flags_before_an_arrival_that_releases_them():
+    """cp.async.mbarrier.arrive tracks copies, not the thread's own stores: the flags that the converting warps read go before
+    the arrival of lane 0, with the warp's barrier between."""
+    src = (CSRC / "sh_attention_kv8.cu").read_text()
+    warp = src[src.index("// ---------------- copies"):src.index("// ---------------- MMA issue")]
+    store, arrive = warp.index("info[2] = ok"), warp.index("mbar_arrive_expect_tx(")
+    assert warp.index("mbar_wait(c_empty") < store < warp.index("__syncwarp()", store) < arrive < warp.index("cp_async_arrive(")
