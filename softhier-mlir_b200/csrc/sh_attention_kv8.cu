@@ -26,7 +26,8 @@ struct KvArgs {
     uint32_t vec;         // q rows take 16-byte loads, o rows 4-byte stores
     uint32_t vec_o;       // o rows take 16-byte stores
     uint32_t box_step, k_at, v_at;      // few rows: bytes from 16 tokens to the next in a stage, K's and V's place there
-    uint32_t boxes, box_bytes;          // few rows: copies per step
+    uint32_t boxes, box_bytes;          // few rows: copies per step, and their bytes
+    uint32_t apart;       // few rows: V comes by a copy of its own, to this place behind K's (0: with K's)
     uint32_t flip;        // sign bits to turn in q: the scale is negative (sl2 is its magnitude then; tiles only)
     uint32_t *counters;   // arrivals per CTA whose last item goes on in others, zero between calls
     float *part;
@@ -201,7 +202,7 @@ struct RowsSmem {
 
 template <int DH, int NT, int NW, bool FP8>
 __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : DH == 64 ? 12 : 8) / NW)
-    k_attn_kv8_rows(const __grid_constant__ CUtensorMap mkv, KvArgs a) {
+    k_attn_kv8_rows(const __grid_constant__ CUtensorMap mkv, const __grid_constant__ CUtensorMap mv, KvArgs a) {
     using SM = RowsSmem<DH, NT, NW>;
     constexpr uint32_t RT = 8 * NT, kThreads = NW * 32;                     // rows of a tile
     constexpr uint32_t kStep = SM::kTokens, kKeys = kStep * NW;             // keys of a warp's step, of a unit
@@ -343,9 +344,12 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : DH == 64 ? 12 : 8) / 
             mbar_arrive_expect_tx(bar, n * a.box_bytes);
 #pragma unroll
             for (uint32_t i = 0; i < HF; ++i)
-                if (i < a.boxes && (uint32_t)id[i] < a.pages)
-                    tma_load_pair(sm + SM::kRing + (warp * kStages + p_slot) * (2 * SM::kTile) + i * SM::kTile, &mkv, bar,
-                                  (int)((p.kvh << a.page_shift) + ((tok + i * 16) & page1)), id[i]);
+                if (i < a.boxes && (uint32_t)id[i] < a.pages) {
+                    uint8_t *dst = sm + SM::kRing + (warp * kStages + p_slot) * (2 * SM::kTile) + i * SM::kTile;
+                    const int row = (int)((p.kvh << a.page_shift) + ((tok + i * 16) & page1));
+                    tma_load_pair(dst, &mkv, bar, row, id[i]);
+                    if (a.apart) tma_load_pair(dst + a.apart, &mv, bar, row, id[i]);
+                }
         }
         p_slot = p_slot + 1 == kStages ? 0 : p_slot + 1;
         advance();
@@ -1289,7 +1293,7 @@ constexpr uint32_t kMaxSms = 160;         // the grid is cut there, so that the 
 constexpr uint64_t kMaxTokens = (1ull << 31) - (1u << 14);
 
 template <int DH, int NT, int NW, bool FP8>
-cudaError_t launch_rows(KvArgs &a, const CUtensorMap &mkv, int sms, cudaStream_t st) {
+cudaError_t launch_rows(KvArgs &a, const CUtensorMap &mkv, const CUtensorMap &mv, int sms, cudaStream_t st) {
     constexpr uint32_t kPerSm = (NT == 1 ? 16 : DH == 64 ? 12 : 8) / NW;
     static_assert(kMaxSms * kPerSm * 4 <= kCounterBytes &&
                       kCounterBytes + (size_t)2 * kPerSm * kMaxSms * 8 * NT * (DH + 2) * 4 <= SH_CUDA_KV8_WS_BYTES,
@@ -1304,7 +1308,7 @@ cudaError_t launch_rows(KvArgs &a, const CUtensorMap &mkv, int sms, cudaStream_t
         if (e != cudaSuccess) return e;
         ready = true;
     }
-    return sh::launch_pdl(kernel, dim3(sms * kPerSm), dim3(NW * 32), RowsSmem<DH, NT, NW>::kBytes, st, mkv, a);
+    return sh::launch_pdl(kernel, dim3(sms * kPerSm), dim3(NW * 32), RowsSmem<DH, NT, NW>::kBytes, st, mkv, mv, a);
 }
 
 template <int DH, bool FP8>
@@ -1343,20 +1347,26 @@ bool kv_map(CUtensorMap *m, uint64_t base, const sh_cuda_kv8_t *c) {
 
 // K and V codes as [2, pages, heads * page, dh] bytes, the lower array first (one of them where both are the same array):
 // boxes of 16 tokens of one page and head, of K and V at once; where pages allow it of the 32 tokens that a step takes.
-bool kv_pair_map(CUtensorMap *m, const sh_cuda_kv8_t *c, KvArgs &a) {
+// Arrays further apart than a map's stride can be (2^40 bytes: two allocators may use address ranges 2^46 apart) get a map each.
+bool kv_pair_map(CUtensorMap *m, CUtensorMap *mv, const sh_cuda_kv8_t *c, KvArgs &a) {
     sh::PFN_encodeTiled enc = sh::encode_tiled();
     if (!enc) return false;
-    const uint32_t step = 2048 / c->dh, rows = step < c->page ? step : c->page, arrays = c->k == c->v ? 1 : 2;
-    a.boxes = step / rows, a.box_bytes = arrays * rows * c->dh, a.box_step = a.boxes == 1 ? 16 * c->dh : 2048;
-    a.k_at = c->k <= c->v ? 0 : rows * c->dh, a.v_at = c->k < c->v ? rows * c->dh : 0;
     const uint64_t lo = c->k < c->v ? c->k : c->v, hi = c->k < c->v ? c->v : c->k;
-    cuuint64_t dims[4] = {c->dh, (cuuint64_t)c->heads * c->page, c->pages, arrays};
-    cuuint64_t strides[3] = {c->dh, c->page_stride, arrays == 2 ? hi - lo : c->page_stride};
-    cuuint32_t box[4] = {c->dh, rows, 1, arrays};
-    cuuint32_t estr[4] = {1, 1, 1, 1};
-    return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, (void *)lo, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               c->dh == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const bool apart = hi - lo >= (1ull << 40);
+    const uint32_t step = 2048 / c->dh, rows = step < c->page ? step : c->page, arrays = lo == hi ? 1 : 2;
+    a.boxes = step / rows, a.box_bytes = arrays * rows * c->dh, a.box_step = a.boxes == 1 ? 16 * c->dh : 2048;
+    a.k_at = c->k <= c->v || apart ? 0 : rows * c->dh, a.v_at = c->k < c->v || apart ? rows * c->dh : 0;
+    a.apart = apart ? rows * c->dh : 0;
+    auto map = [&](CUtensorMap *to, uint64_t base, uint32_t n) {
+        cuuint64_t dims[4] = {c->dh, (cuuint64_t)c->heads * c->page, c->pages, n};
+        cuuint64_t strides[3] = {c->dh, c->page_stride, n == 2 ? hi - lo : c->page_stride};
+        cuuint32_t box[4] = {c->dh, rows, 1, n};
+        cuuint32_t estr[4] = {1, 1, 1, 1};
+        return enc(to, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, (void *)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   c->dh == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    };
+    return apart ? map(m, c->k, 1) && map(mv, c->v, 1) : map(m, lo, arrays);
 }
 
 }  // namespace
@@ -1401,8 +1411,8 @@ int sh_cuda_attention_kv8(uint64_t q, uint64_t o, const sh_cuda_kv8_t *c, uint64
     const int sms = s.num_sms < (int)kMaxSms ? s.num_sms : (int)kMaxSms;
     const bool fp8 = c->fmt == SH_FP8, wide = (uint64_t)max_q * a.G > 8;
     const bool tall = (uint64_t)max_q * a.G > 64;
-    CUtensorMap mk, mv;
-    if (tall ? !kv_map(&mk, c->k, c) || !kv_map(&mv, c->v, c) : !kv_pair_map(&mk, c, a)) {
+    CUtensorMap mk, mv = {};
+    if (tall ? !kv_map(&mk, c->k, c) || !kv_map(&mv, c->v, c) : !kv_pair_map(&mk, &mv, c, a)) {
         sh::set_error(-1, "[sh_cuda_attention_kv8] no tensor map for the cache (page_stride=%llu)",
                       (unsigned long long)c->page_stride);
         return -1;
@@ -1413,7 +1423,7 @@ int sh_cuda_attention_kv8(uint64_t q, uint64_t o, const sh_cuda_kv8_t *c, uint64
     // the others go on while one ends an item (64 requests of up to 8192 tokens 115 us, 123 us with eight).
     const bool few = (uint64_t)R * c->heads < (uint64_t)sms;
 #define SH_KV8(dh, nt, n) \
-    (fp8 ? launch_rows<dh, nt, n, true>(a, mk, sms, s.stream) : launch_rows<dh, nt, n, false>(a, mk, sms, s.stream))
+    (fp8 ? launch_rows<dh, nt, n, true>(a, mk, mv, sms, s.stream) : launch_rows<dh, nt, n, false>(a, mk, mv, sms, s.stream))
     // 64 rows are four tiles of the kernel above: 16 requests of 7 drafts (28 rows) 77 us there, 128 us here; 4 of 64 (256 rows)
     // 126 us there, 73 us here.
     if (tall) {

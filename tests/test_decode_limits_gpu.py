@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from oracle import decode as D
-from softhier_cuda import lib as L
+from softhier_cuda import decode, lib as L
 from test_decode_gpu import DEV, Pool, _attn_tol, _i32, _np, _p
 
 pytestmark = pytest.mark.gpu
@@ -118,3 +118,87 @@ def test_attention_of_a_length_past_the_table(gpu_lib, nq, over):
     err = np.abs(_np(do).astype(np.float64) - want)
     tol = _attn_tol(want, mean_abs, big, keys, H, dh, vmax)
     assert (err <= tol).all(), np.argwhere(err > tol)[:4]
+
+
+# ---- K and V far apart ----------------------------------------------------------------------------------------------------
+class FarMemory:
+    """`size` bytes of device memory at an address at least 2^41 bytes away from `other` (virtual memory management of the
+    driver: reserve, create, map), as a second allocator may give them."""
+
+    def __init__(self, size, other):
+        import ctypes as C
+        self.C, self.cu = C, C.CDLL("libcuda.so.1")
+
+        class Location(C.Structure):
+            _fields_ = [("type", C.c_int), ("id", C.c_int)]
+
+        class Prop(C.Structure):
+            _fields_ = [("type", C.c_int), ("handles", C.c_int), ("location", Location), ("win32", C.c_void_p),
+                        ("flags", C.c_ubyte * 8)]
+
+        class Access(C.Structure):
+            _fields_ = [("location", Location), ("flags", C.c_int)]
+        loc = Location(1, torch.cuda.current_device())             # a device, pinned memory, read and write
+        self.ptr = self.handle = None
+        self.size, self.reserved = -(-size // (1 << 21)) * (1 << 21), 1 << 30
+        for hint in (0, 1 << 45, other - (1 << 42) >> 21 << 21):
+            p = C.c_uint64()
+            if self.cu.cuMemAddressReserve(C.byref(p), C.c_size_t(self.reserved), C.c_size_t(0), C.c_uint64(hint), C.c_ulonglong(0)):
+                continue
+            if abs(p.value - other) >= 1 << 41:
+                self.ptr = p.value
+                break
+            self.cu.cuMemAddressFree(p, C.c_size_t(self.reserved))
+        if self.ptr is None:
+            pytest.skip("the driver gives no address that far away")
+        h = C.c_uint64()
+        assert self.cu.cuMemCreate(C.byref(h), C.c_size_t(self.size), C.byref(Prop(1, 0, loc)), C.c_ulonglong(0)) == 0
+        self.handle = h
+        assert self.cu.cuMemMap(C.c_uint64(self.ptr), C.c_size_t(self.size), C.c_size_t(0), h, C.c_ulonglong(0)) == 0
+        assert self.cu.cuMemSetAccess(C.c_uint64(self.ptr), C.c_size_t(self.size), C.byref(Access(loc, 3)), C.c_size_t(1)) == 0
+
+    def free(self):
+        C = self.C
+        torch.cuda.synchronize()
+        assert self.cu.cuMemUnmap(C.c_uint64(self.ptr), C.c_size_t(self.size)) == 0
+        assert self.cu.cuMemRelease(self.handle) == 0
+        assert self.cu.cuMemAddressFree(C.c_uint64(self.ptr), C.c_size_t(self.reserved)) == 0
+
+
+@pytest.mark.parametrize("fmt,page,dh", [("int8", 16, 64), ("fp8", 64, 64), ("fp8", 16, 128), ("int8", 128, 128)])
+def test_attention_of_arrays_in_different_address_ranges(gpu_lib, fmt, page, dh):
+    """K and V more than 2^40 bytes apart, either first: the bits of the same cache with both side by side."""
+    rt = gpu_lib
+    H, heads = 8, 2
+    lens = np.array([300, 1, 77, 33])
+    blocks = -(-lens // page)
+    pool = Pool(int(blocks.sum()), heads, page, dh, fmt, 3)
+    size = int(np.prod(pool.shape))
+    table = np.zeros((4, int(blocks.max())), np.int64)
+    for r in range(4):
+        table[r, :blocks[r]] = blocks[:r].sum() + np.arange(blocks[r])
+    far = FarMemory(size, _p(pool.raw))
+    try:
+        for near_k in (True, False):
+            for nq in ((1, 1, 1, 1), (5, 1, 0, 7), (100, 1, 20, 33)):
+                T, start = sum(nq), _i32(np.concatenate([[0], np.cumsum(nq)]))
+                q = torch.randn((T, H * dh), device=DEV, generator=torch.Generator(DEV).manual_seed(T)).half()
+                ws = torch.zeros(L.KV8_WS_BYTES, dtype=torch.uint8, device=DEV)
+                d_table, d_lens, outs = _i32(table), _i32(lens), []
+                for apart in (False, True):
+                    k, v = _p(pool.raw), _p(pool.raw) + size
+                    if apart:
+                        src = v if near_k else k
+                        assert rt.lib.sh_cuda_copy2d(far.ptr, size, src, size, size, 1, rt.lib.sh_cuda_get_stream()) == 0
+                        k, v = (k, far.ptr) if near_k else (far.ptr, v)
+                    h = L.Kv8(k, v, _p(pool.dev_scales[0]), _p(pool.dev_scales[1]), pool.stride, pool.shape[0], page, heads, dh,
+                              decode.FORMATS[fmt])
+                    o = torch.full_like(q, 7.0)
+                    rc = rt.lib.sh_cuda_attention_kv8(_p(q), _p(o), h, _p(d_table), table.shape[1], _p(d_lens), _p(start), 4, T, max(nq),
+                                                      H, H * dh, H * dh, 0.125, _p(ws), ws.numel())
+                    assert rc == 0
+                    rt.check()
+                    outs.append(_np(o).view(np.uint16))
+                np.testing.assert_array_equal(outs[0], outs[1])
+    finally:
+        far.free()
