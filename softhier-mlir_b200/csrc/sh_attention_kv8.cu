@@ -1299,35 +1299,29 @@ cudaError_t launch_rows(KvArgs &a, const CUtensorMap &mkv, const CUtensorMap &mv
                       kCounterBytes + (size_t)2 * kPerSm * kMaxSms * 8 * NT * (DH + 2) * 4 <= SH_CUDA_KV8_WS_BYTES,
                   "workspace: a counter and two partial items per CTA");
     static_assert(kPerSm * (RowsSmem<DH, NT, NW>::kBytes + 1024) <= 228 * 1024, "shared memory of the CTAs of an SM");
-    auto kernel = k_attn_kv8_rows<DH, NT, NW, FP8>;
-    static bool done[sh::kMaxDevices] = {};
-    bool &ready = done[sh::current_device() % sh::kMaxDevices];
-    if (!ready) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   RowsSmem<DH, NT, NW>::kBytes);
-        if (e != cudaSuccess) return e;
-        ready = true;
-    }
-    return sh::launch_pdl(kernel, dim3(sms * kPerSm), dim3(NW * 32), RowsSmem<DH, NT, NW>::kBytes, st, mkv, mv, a);
+    const cudaError_t e = sh::allow_smem<k_attn_kv8_rows<DH, NT, NW, FP8>>(RowsSmem<DH, NT, NW>::kBytes);
+    if (e != cudaSuccess) return e;
+    return sh::launch_pdl(k_attn_kv8_rows<DH, NT, NW, FP8>, dim3(sms * kPerSm), dim3(NW * 32), RowsSmem<DH, NT, NW>::kBytes, st,
+                          mkv, mv, a);
 }
 
 template <int DH, bool FP8>
 cudaError_t launch_tiles(KvArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int sms, cudaStream_t st) {
     static_assert(kCounterBytes + (size_t)2 * kMaxSms * kTlItem * (DH + 2) * 4 <= SH_CUDA_KV8_WS_BYTES,
                   "workspace: two partial items per CTA");
-    auto kernel = k_attn_kv8_tiles<DH, FP8>;
+    constexpr auto kernel = k_attn_kv8_tiles<DH, FP8>;
     // the kernel hands registers from warp to warp: it has to start with as many as it ends with
     static_assert(512 * kTlRegs + (kTlThreads - 512) * kTlRegsOther <= kTlThreads * 80, "registers");
-    static bool done[sh::kMaxDevices] = {};
-    bool &ready = done[sh::current_device() % sh::kMaxDevices];
-    if (!ready) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TilesSmem<DH>::kBytes);
-        if (e != cudaSuccess) return e;
+    static std::atomic<bool> enough[sh::kMaxDevices];
+    std::atomic<bool> &ok = enough[sh::current_device() % sh::kMaxDevices];
+    cudaError_t e = sh::allow_smem<kernel>(TilesSmem<DH>::kBytes);
+    if (e != cudaSuccess) return e;
+    if (!ok.load(std::memory_order_relaxed)) {
         cudaFuncAttributes at;
         e = cudaFuncGetAttributes(&at, kernel);
         if (e != cudaSuccess) return e;
         if (at.numRegs < 80) return cudaErrorInvalidDeviceFunction;
-        ready = true;
+        ok.store(true, std::memory_order_relaxed);
     }
     return sh::launch_pdl(kernel, dim3(sms), dim3(kTlThreads), TilesSmem<DH>::kBytes, st, mk, mv, a);
 }

@@ -569,13 +569,9 @@ cudaError_t w4_try(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bo
     // K parts over a cluster while the columns alone leave SMs idle and every warp keeps a step, or until X fits
     a.staged = (((uint64_t)a.scales | (uint64_t)a.zeros) & 15) == 0 && a.K % kUnit == 0 && a.K / G * 96 <= kMaxScales / NG;
     auto kernel = a.zeros ? k_gemv_w4<G, INT, NT, NG, D, true> : k_gemv_w4<G, INT, NT, NG, D, false>;
-    static bool done[2][sh::kMaxDevices] = {};
-    bool &ready = done[a.zeros != nullptr][sh::current_device() % sh::kMaxDevices];
-    if (!ready) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax);
-        if (e != cudaSuccess) return e;
-        ready = true;
-    }
+    const cudaError_t e = a.zeros ? sh::allow_smem<k_gemv_w4<G, INT, NT, NG, D, true>>(kSmemMax)
+                                  : sh::allow_smem<k_gemv_w4<G, INT, NT, NG, D, false>>(kSmemMax);
+    if (e != cudaSuccess) return e;
     for (;; s *= 2) {
         room = w4_clusters(kernel, NG * kGroupThreads, s, (uint32_t)sms);
         const uint32_t ctas = tiles < room ? tiles : room;

@@ -40,3 +40,11 @@ def test_the_copy_warp_stores_a_stages_flags_before_an_arrival_that_releases_the
     warp = src[src.index("// ---------------- copies"):src.index("// ---------------- MMA issue")]
     store, arrive = warp.index("info[2] = ok"), warp.index("mbar_arrive_expect_tx(")
     assert warp.index("mbar_wait(c_empty") < store < warp.index("__syncwarp()", store) < arrive < warp.index("cp_async_arrive(")
+
+
+@pytest.mark.parametrize("name", ["sh_kvcache.cu", "sh_attention_kv8.cu", "sh_gemv_w4.cu", "sh_kv8.cuh"])
+def test_what_decode_calls_remember_per_device_is_atomic(name):
+    """Several host threads may make their first calls at the same time."""
+    lines = [ln.strip() for ln in (CSRC / name).read_text().splitlines()]
+    kept = [ln for ln in lines if ln.startswith("static ") and "static_assert" not in ln and "constexpr" not in ln]
+    assert all("std::atomic<" in ln for ln in kept), kept
