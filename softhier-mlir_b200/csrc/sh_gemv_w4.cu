@@ -23,8 +23,6 @@
 // instruction is free when both operands agree. A tile's scales and zero points come as rows of 16 bytes, one tile
 // ahead. When the columns alone do not fill the GPU, the CTAs of a cluster share K. All partial sums meet in shared
 // memory in a fixed order.
-#include <atomic>
-
 #include "sh_internal.cuh"
 
 namespace {
@@ -538,27 +536,30 @@ bool w4_map(CUtensorMap *m, uint64_t codes, uint32_t N, uint32_t K, uint32_t ldw
 
 constexpr size_t kSmemMax = 227 * 1024, kMaxScales = 64 * 1024;
 
-// Clusters of s CTAs (one per SM) that run at once: the GPU's SMs come in groups that a cluster does not cross, so there are
-// fewer than num_sms / s of them (33 of 4, not 37), and one more would be a second wave. A property of the device, asked once.
-template <typename K>
-uint32_t w4_clusters(K kernel, uint32_t threads, uint32_t s, uint32_t sms) {
+// Clusters of s CTAs (one per SM) of a kernel that run at once: the GPU's SMs come in groups that a cluster does not cross, so
+// there are fewer than num_sms / s of them (33 of 4, not 37), and one more would be a second wave. Asked once per kernel and
+// device; when the runtime gives no answer the next call asks again.
+template <auto Kernel>
+uint32_t w4_clusters(uint32_t threads, uint32_t s, uint32_t sms) {
     if (s == 1) return sms;
     static std::atomic<uint32_t> known[sh::kMaxDevices][9];      // s is 2, 4 or 8
-    std::atomic<uint32_t> &k = known[sh::state().device % sh::kMaxDevices][s];
-    uint32_t n = k.load(std::memory_order_relaxed);
-    if (n == 0) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(1, s), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = kSmemMax;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = 1, attr[0].val.clusterDim.y = s, attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr, cfg.numAttrs = 1;
-        int got = 0;
-        n = sms / s;
-        if (cudaOccupancyMaxActiveClusters(&got, kernel, &cfg) == cudaSuccess && got > 0 && (uint32_t)got < n) n = (uint32_t)got;
-        k.store(n, std::memory_order_relaxed);
+    std::atomic<uint32_t> &k = known[sh::current_device() % sh::kMaxDevices][s];
+    const uint32_t n = k.load(std::memory_order_relaxed);
+    if (n) return n;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1, s), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = kSmemMax;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1, attr[0].val.clusterDim.y = s, attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    int got = 0;
+    if (cudaOccupancyMaxActiveClusters(&got, Kernel, &cfg) != cudaSuccess || got <= 0) {
+        cudaGetLastError();
+        return sms / s;
     }
-    return n;
+    const uint32_t most = (uint32_t)got < sms / s ? (uint32_t)got : sms / s;
+    k.store(most, std::memory_order_relaxed);
+    return most;
 }
 
 template <int G, bool INT, int NT, int NG, int D>
@@ -573,7 +574,8 @@ cudaError_t w4_try(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bo
                                   : sh::allow_smem<k_gemv_w4<G, INT, NT, NG, D, false>>(kSmemMax);
     if (e != cudaSuccess) return e;
     for (;; s *= 2) {
-        room = w4_clusters(kernel, NG * kGroupThreads, s, (uint32_t)sms);
+        room = a.zeros ? w4_clusters<k_gemv_w4<G, INT, NT, NG, D, true>>(NG * kGroupThreads, s, (uint32_t)sms)
+                       : w4_clusters<k_gemv_w4<G, INT, NT, NG, D, false>>(NG * kGroupThreads, s, (uint32_t)sms);
         const uint32_t ctas = tiles < room ? tiles : room;
         iters = s > 1 ? (tiles + ctas * NG - 1) / (ctas * NG) : 0;      // sums kept for the cluster
         smem = w4_layout(NG, D, NT, kUnit / G, INT, a.zeros != nullptr, (units + s - 1) / s + 1, a.M,

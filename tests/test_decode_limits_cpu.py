@@ -48,3 +48,12 @@ def test_what_decode_calls_remember_per_device_is_atomic(name):
     lines = [ln.strip() for ln in (CSRC / name).read_text().splitlines()]
     kept = [ln for ln in lines if ln.startswith("static ") and "static_assert" not in ln and "constexpr" not in ln]
     assert all("std::atomic<" in ln for ln in kept), kept
+
+
+def test_cluster_counts_are_kept_per_kernel_and_only_when_the_runtime_gave_them():
+    """All forms of the kernel have one function type, so a table in a function over that type would be one for all of them."""
+    src = (CSRC / "sh_gemv_w4.cu").read_text()
+    fn = src[src.index("w4_clusters(") - 40:src.index("cudaError_t w4_try")]
+    assert "template <auto Kernel>" in fn and fn.count(".store(") == 1
+    failed = fn.index("!= cudaSuccess")
+    assert failed < fn.index("return sms / s;", failed) < fn.index(".store(")
