@@ -445,9 +445,8 @@ __global__ void __launch_bounds__(kAppThreads) k_kv8_append(AppendArgs a) {
 }
 
 template <int DH, bool FP8>
-void append_launch(const AppendArgs &a, bool vec, dim3 grid, cudaStream_t st) {
-    if (vec) sh::launch_pdl(k_kv8_append<DH, FP8, true>, grid, dim3(kAppThreads), 0, st, a);
-    else sh::launch_pdl(k_kv8_append<DH, FP8, false>, grid, dim3(kAppThreads), 0, st, a);
+cudaError_t append_launch(const AppendArgs &a, bool vec, dim3 grid, cudaStream_t st) {
+    return sh::launch_pdl(vec ? k_kv8_append<DH, FP8, true> : k_kv8_append<DH, FP8, false>, grid, dim3(kAppThreads), 0, st, a);
 }
 
 }  // namespace
@@ -516,9 +515,9 @@ int sh_cuda_kv8_append(const sh_cuda_kv8_t *c, uint64_t k, uint64_t v, uint32_t 
     const bool vec = sh::aligned16(k) && sh::aligned16(v) && ldk % 8 == 0 && ldv % 8 == 0;
     const dim3 grid(gx, c->heads * 2);
     const bool fp8 = c->fmt == SH_FP8;
-    if (c->dh == 64) fp8 ? append_launch<64, true>(a, vec, grid, s.stream) : append_launch<64, false>(a, vec, grid, s.stream);
-    else fp8 ? append_launch<128, true>(a, vec, grid, s.stream) : append_launch<128, false>(a, vec, grid, s.stream);
-    return sh::cuda_ok(cudaGetLastError(), "sh_cuda_kv8_append") ? 0 : -1;
+    auto launch = c->dh == 64 ? (fp8 ? append_launch<64, true> : append_launch<64, false>)
+                              : (fp8 ? append_launch<128, true> : append_launch<128, false>);
+    return sh::cuda_ok(launch(a, vec, grid, s.stream), "sh_cuda_kv8_append") ? 0 : -1;
 }
 
 }  // extern "C"

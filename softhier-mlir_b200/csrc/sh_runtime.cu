@@ -53,6 +53,7 @@ void set_error(int code, const char *fmt, ...) {
 
 bool cuda_ok(cudaError_t e, const char *where) {
     if (e == cudaSuccess) return true;
+    cudaGetLastError();      // reported here: the next call's own check must not find it again
     set_error((int)e, "[sh_cuda] %s: %s", where, cudaGetErrorString(e));
     return false;
 }

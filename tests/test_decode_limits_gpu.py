@@ -202,3 +202,17 @@ def test_attention_of_arrays_in_different_address_ranges(gpu_lib, fmt, page, dh)
                 np.testing.assert_array_equal(outs[0], outs[1])
     finally:
         far.free()
+
+
+# ---- after a failed call ----------------------------------------------------------------------------------------------------
+def test_append_after_a_failed_call(gpu_lib, capfd):
+    """A CUDA call of the library that was refused before, and reported, is not reported as this one's."""
+    rt = gpu_lib
+    pool = Pool(4, 2, 16, 64, "int8", 2)
+    x, s = torch.ones((1, 128), dtype=torch.float16, device=DEV), _i32([5])
+    rt.check()
+    assert not rt.lib.sh_cuda_ipc_alloc(1 << 50)           # more memory than there is
+    assert rt.lib.sh_cuda_kv8_append(pool.handle, _p(x), _p(x), 1, 128, 128, _p(s)) == 0
+    assert rt.lib.sh_cuda_last_error() != 0 and rt.lib.sh_cuda_last_error() == 0
+    rt.check()
+    capfd.readouterr()
