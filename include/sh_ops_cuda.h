@@ -175,8 +175,9 @@ int sh_cuda_kv8_append(const sh_cuda_kv8_t *cache, uint64_t k, uint64_t v, uint3
 /* Attention of the new rows of R requests over the cache: row q_start[r] + i of q (i < q_start[r + 1] - q_start[r] = n)
  * is a query of request r, which has lens[r] tokens in the cache, these n last, and attends its tokens
  * j <= lens[r] - n + i; query head h reads head h / (H / heads) of the cache. o = softmax(scale q k^T) v in the rows of q,
- * fp16 (leading dims ldq, ldo); a row without any token gives zeros; rows of o outside [q_start[0], q_start[R]) and past T
- * are left as they were. One token per request, a few drafted ones, and whole prompt chunks are all
+ * fp16 (leading dims ldq, ldo); a row without any token gives zeros, an infinity or a NaN in a row of q NaN in its head
+ * (where the row has a token); rows of o outside [q_start[0], q_start[R]) and past T are left as they were. One token per
+ * request, a few drafted ones, and whole prompt chunks are all
  * served, in any mixture. q holds T rows; max_q, the most rows of one request, only picks the kernel (a wrong value
  * costs time). ws: ws_bytes >= SH_CUDA_KV8_WS_BYTES of device memory, 16-byte aligned, zeroed once before its first use,
  * for the calls of one stream at a time (a graph that may run beside other calls has its own). A table entry outside the

@@ -53,6 +53,20 @@ __device__ __forceinline__ ReqView req_view(const KvArgs &a, uint32_t r) {
     return v;
 }
 
+// The sum of weights of a row, from token `first` on, that came out as 0: 0 when the row has no keys there (none at all gives
+// zeros). Scores that are all -infinity, from an infinity in Q beside keys of one sign, give NaN as beside keys of both signs;
+// they are rare, so that Q is looked at here only.
+__device__ __forceinline__ float no_weight(const KvArgs &a, const ReqView &v, uint32_t kvh, uint32_t row, uint32_t dh,
+                                           uint32_t first) {
+    const uint32_t qi = row / a.G, gi = row - qi * a.G;
+    if (min(v.base + (int)qi + 1, (int)v.ctx) <= (int)first) return 0.f;
+    const __half *q = a.q + (size_t)(v.qs + qi) * a.ldq + ((size_t)kvh * a.G + gi) * dh;
+#pragma unroll 1
+    for (uint32_t d = 0; d < dh; ++d)
+        if ((__half_as_ushort(q[d]) & 0x7FFFu) == 0x7C00u) return NAN;
+    return 0.f;
+}
+
 __device__ __forceinline__ uint4 lds16(uint32_t at) {
     uint4 r;
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
@@ -575,6 +589,7 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : DH == 64 ? 12 : 8) / 
                     ll = fmaf(s_l[w * RT + t], f, ll);
                     s_m[w * RT + t] = f;
                 }
+                if (ll == 0.f && t < nrows) ll = no_weight(a, v, kvh, row0 + t, DH, b0 * kKeys);
                 s_l[t] = ll, s_l[RT + t] = mx;
             }
             __syncthreads();
@@ -608,6 +623,7 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : DH == 64 ? 12 : 8) / 
                 x = fmaf(p.x, f, x);
                 y = fmaf(p.y, f, y);
             }
+            if (NT == 1 && ll == 0.f) ll = no_weight(a, v, kvh, row0 + n, DH, b0 * kKeys);
             if (whole) {
                 write_out(n, d, x, y, ll);
             } else {
@@ -1178,6 +1194,7 @@ __global__ void __launch_bounds__(kTlThreads, 1)
                 row_sum[half * 128] = l;
                 tile_sync();
                 l = row_sum[0] + row_sum[128];
+                if (l == 0.f && mine) l = no_weight(a, k.v, k.kvh, k.row0 + rr, DH, b0 * kTlKeys);
                 tile_sync();      // read before the next item's Q goes there
             }
             const bool whole = b0 == 0 && nb == k.blocks;

@@ -1,6 +1,7 @@
 """The decode-step operators at the edges of what their header allows."""
 from __future__ import annotations
 
+import math
 import subprocess
 import sys
 from pathlib import Path
@@ -216,3 +217,37 @@ def test_append_after_a_failed_call(gpu_lib, capfd):
     assert rt.lib.sh_cuda_last_error() != 0 and rt.lib.sh_cuda_last_error() == 0
     rt.check()
     capfd.readouterr()
+
+
+# ---- queries that are not finite ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("nq", [1, 12, 80])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_attention_of_infinite_queries_is_nan_whatever_the_keys(gpu_lib, fmt, nq, value):
+    """Also where every key has the same sign in that column, so that all scores are +infinity or all -infinity; a row without keys
+    stays zero."""
+    rt = gpu_lib
+    pool = Pool(8, 2, 32, 64, fmt, 4)
+    pool.codes[0][..., 9] = D.encode(np.array(3.0), fmt)
+    pool.raw.copy_(torch.from_numpy(np.stack(pool.codes).reshape(-1)))
+    q = torch.randn((2 * nq, 256), device=DEV, generator=torch.Generator(DEV).manual_seed(1)).half()
+    start, table, lens = _i32([0, nq, 2 * nq]), _i32([[0, 1, 2, 3], [4, 5, 6, 7]]), _i32([nq - 1, 100])
+    ws = torch.zeros(L.KV8_WS_BYTES, dtype=torch.uint8, device=DEV)
+
+    def run(x):
+        o = torch.zeros_like(x)
+        assert rt.lib.sh_cuda_attention_kv8(_p(x), _p(o), pool.handle, _p(table), 4, _p(lens), _p(start), 2, 2 * nq, nq, 4, 256, 256,
+                                            0.125, _p(ws), ws.numel()) == 0
+        rt.check()
+        return _np(o).reshape(2 * nq, 4, 64)
+    good = run(q)
+    rows = sorted({0, nq - 1, nq, 2 * nq - 1})
+    x = q.clone()
+    for r in rows:
+        x[r, 64 + 9] = value
+    got = run(x)
+    hit = np.zeros(good.shape[:2], bool)
+    for r in rows:
+        hit[r, 1] = r > 0           # row 0 has no key
+    assert np.isnan(got[hit]).all() and (got[0] == 0).all()
+    assert np.array_equal(got[~hit].view(np.uint16), good[~hit].view(np.uint16))
