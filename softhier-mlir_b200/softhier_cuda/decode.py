@@ -44,8 +44,15 @@ class KvCache:
             _lib.Kv8(self.codes[i, 0].data_ptr(), self.codes[i, 1].data_ptr(), self.scales[i, 0].data_ptr(),
                      self.scales[i, 1].data_ptr(), heads * page * dh, pages, page, heads, dh, FORMATS[fmt])
             for i in range(layers)]
+        torch.cuda.synchronize(rt.device)      # filled on torch's current stream, used on the library's, whichever that is
 
-    def _must(self, rc: int) -> None:
+    def _call(self, fn, *args) -> None:
+        """The library works on the calling thread's current device, which may be another runtime's."""
+        if torch.cuda.current_device() == self.rt.device:
+            rc = fn(*args)
+        else:
+            with torch.cuda.device(self.rt.device):
+                rc = fn(*args)
         if rc:
             raise ShCudaError(f"libsh_ops_cuda error {rc}: {self.rt.lib.sh_cuda_last_error_string().decode()}")
 
@@ -54,22 +61,22 @@ class KvCache:
         if add.dtype != torch.int32 or add.shape != self.lens.shape or add.device != self.lens.device or not add.is_contiguous():
             raise ShCudaError(f"add is not a contiguous int32 [{self.requests}] on {self.lens.device}")
         p = torch.Tensor.data_ptr
-        self._must(self.rt.lib.sh_cuda_kv_tables(
-            p(self.lens), p(add), self.requests, self.page, p(self.table), self.blocks, p(self.ring), self.pages,
-            p(self.pool), p(self.pool), p(self.lens), p(self.q_start), p(self.slots), p(self.pos), self.t_cap))
+        self._call(self.rt.lib.sh_cuda_kv_tables,
+                   p(self.lens), p(add), self.requests, self.page, p(self.table), self.blocks, p(self.ring), self.pages,
+                   p(self.pool), p(self.pool), p(self.lens), p(self.q_start), p(self.slots), p(self.pos), self.t_cap)
 
     def append(self, layer: int, k: int, v: int, ldk: int, ldv: int, T: int) -> None:
         """k, v: device addresses of fp16 [T, heads * dh]."""
         if T > self.t_cap:
             raise ShCudaError(f"{T} rows in a step of at most {self.t_cap}")
-        self._must(self.rt.lib.sh_cuda_kv8_append(self.handles[layer], k, v, T, ldk, ldv, self.slots.data_ptr()))
+        self._call(self.rt.lib.sh_cuda_kv8_append, self.handles[layer], k, v, T, ldk, ldv, self.slots.data_ptr())
 
     def attend(self, layer: int, q: int, o: int, T: int, H: int, ldq: int, ldo: int, scale: float, max_q: int = 1) -> None:
         """q, o: device addresses of fp16 [T, H * dh]."""
         p = torch.Tensor.data_ptr
-        self._must(self.rt.lib.sh_cuda_attention_kv8(
-            q, o, self.handles[layer], p(self.table), self.blocks, p(self.lens), p(self.q_start), self.requests, T, max_q,
-            H, ldq, ldo, scale, p(self.ws), self.ws.numel()))
+        self._call(self.rt.lib.sh_cuda_attention_kv8,
+                   q, o, self.handles[layer], p(self.table), self.blocks, p(self.lens), p(self.q_start), self.requests, T,
+                   max_q, H, ldq, ldo, scale, p(self.ws), self.ws.numel())
 
 
 def quantize_w4(w: np.ndarray, group: int, symmetric: bool = False):

@@ -2,10 +2,12 @@
 from __future__ import annotations
 
 from pathlib import Path
+from types import SimpleNamespace
 
 import pytest
+import torch
 
-from softhier_cuda import lib as L
+from softhier_cuda import decode, lib as L
 from test_decode_cpu import _attn, _cache, lib  # noqa: F401  (lib: the fixture)
 
 CSRC = Path(__file__).resolve().parents[1] / "softhier-mlir_b200" / "csrc"
@@ -57,3 +59,37 @@ def test_cluster_counts_are_kept_per_kernel_and_only_when_the_runtime_gave_them(
     assert "template <auto Kernel>" in fn and fn.count(".store(") == 1
     failed = fn.index("!= cudaSuccess")
     assert failed < fn.index("return sms / s;", failed) < fn.index(".store(")
+
+
+def test_a_cache_is_filled_before_and_used_on_its_own_device(monkeypatch):
+    """The tensors are filled on torch's stream and used on the library's: the constructor waits for them. A call that finds another
+    device current (a second runtime's) is made on the cache's."""
+    now, waits, calls = [1], [], []
+
+    class Device:
+        def __init__(self, d):
+            self.d = d
+
+        def __enter__(self):
+            self.old, now[0] = now[0], self.d
+
+        def __exit__(self, *exc):
+            now[0] = self.old
+
+    for name in ("zeros", "arange"):
+        make = getattr(torch, name)
+        monkeypatch.setattr(torch, name, lambda *a, make=make, device=None, **k: make(*a, **k))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda d=None: waits.append((d, len(calls))))
+    lib_ = SimpleNamespace(**{n: (lambda *a, n=n: calls.append((n, now[0])) or 0) for n in (
+        "sh_cuda_kv_tables", "sh_cuda_kv8_append", "sh_cuda_attention_kv8")})
+    cache = decode.KvCache(SimpleNamespace(device=0, lib=lib_), layers=1, heads=2, dh=64, page=16, pages=8, requests=3, blocks=2)
+    assert waits == [(0, 0)]
+    for current in (1, 0):
+        now[0] = current
+        cache.step(torch.ones(3, dtype=torch.int32))
+        cache.append(0, 256, 256, 128, 128, 3)
+        cache.attend(0, 256, 256, 3, 4, 256, 256, 0.125)
+        assert now[0] == current
+    assert [d for _, d in calls] == [0] * 6 and len({n for n, _ in calls}) == 3

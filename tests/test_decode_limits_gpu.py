@@ -251,3 +251,22 @@ def test_attention_of_infinite_queries_is_nan_whatever_the_keys(gpu_lib, fmt, nq
         hit[r, 1] = r > 0           # row 0 has no key
     assert np.isnan(got[hit]).all() and (got[0] == 0).all()
     assert np.array_equal(got[~hit].view(np.uint16), good[~hit].view(np.uint16))
+
+
+# ---- the host side ------------------------------------------------------------------------------------------------------------
+def test_cache_made_while_torchs_stream_is_busy(gpu_lib):
+    """A new cache is used on another stream at once, while torch's own stream, which fills it, had work to do."""
+    rt, old, side = gpu_lib, gpu_lib.stream, torch.cuda.Stream()
+    add = _i32([3, 0, 2])
+    torch.cuda.synchronize()
+    try:
+        rt.activate(side)
+        torch.cuda._sleep(100_000_000)
+        cache = decode.KvCache(rt, layers=1, heads=2, dh=64, page=16, pages=8, requests=3, blocks=2, t_cap=8)
+        cache.step(add)
+        rt.check()
+    finally:
+        rt.activate(old)
+    torch.cuda.synchronize()
+    assert cache.lens.tolist() == [3, 0, 2] and cache.pool[:3].tolist() == [2, 6, 0]
+    assert cache.slots.tolist() == [0, 1, 2, 16, 17, -1, -1, -1]
