@@ -79,6 +79,13 @@ class KvCache:
                    max_q, H, ldq, ldo, scale, p(self.ws), self.ws.numel())
 
 
+def _w4_scales(step: np.ndarray) -> np.ndarray:
+    """fp16, nearest; below fp16's normal range, where nearest may lose any part of a step, not less than the step, so that 15 of
+    them still cover the group."""
+    s = step.astype(np.float16)
+    return np.where((s < 2.0 ** -14) & (s.astype(np.float32) < step), np.nextafter(s, np.float16(1)), s)
+
+
 def quantize_w4(w: np.ndarray, group: int, symmetric: bool = False):
     """W [K, N] -> (codes uint8 [N, K / 2 padded to 16 bytes], scales fp16 [N, K / group], zeros uint8 or None) of
     sh_cuda_gemv_w4. Per output column and group: from the smallest to the largest value in 15 steps, or with `symmetric`
@@ -90,12 +97,12 @@ def quantize_w4(w: np.ndarray, group: int, symmetric: bool = False):
     if not np.abs(x).max(initial=0.0) <= 65504.0:
         raise ValueError("a weight is not finite or beyond fp16")
     if symmetric:
-        scales = (np.abs(x).max(2) / 7.0).astype(np.float16)
+        scales = _w4_scales(np.abs(x).max(2) / np.float32(7.0))
         zeros = None
         z = np.float32(8.0)
     else:
         lo, hi = np.minimum(x.min(2), 0.0), np.maximum(x.max(2), 0.0)
-        scales = ((hi - lo) / 15.0).astype(np.float16)
+        scales = _w4_scales((hi - lo) / np.float32(15.0))
         s = np.where(scales > 0, scales, 1).astype(np.float32)
         zeros = np.clip(np.rint(-lo / s), 0, 15).astype(np.uint8)
         z = zeros.astype(np.float32)[:, :, None]

@@ -4,9 +4,11 @@ from __future__ import annotations
 from pathlib import Path
 from types import SimpleNamespace
 
+import numpy as np
 import pytest
 import torch
 
+from oracle import decode as D
 from softhier_cuda import decode, lib as L
 from test_decode_cpu import _attn, _cache, lib  # noqa: F401  (lib: the fixture)
 
@@ -93,3 +95,18 @@ def test_a_cache_is_filled_before_and_used_on_its_own_device(monkeypatch):
         cache.attend(0, 256, 256, 3, 4, 256, 256, 0.125)
         assert now[0] == current
     assert [d for _, d in calls] == [0] * 6 and len({n for n, _ in calls}) == 3
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-4, 1e-5, 1e-6, 2e-7, 1e-7, 1e-8])
+@pytest.mark.parametrize("symmetric", [False, True])
+def test_quantize_w4_covers_groups_of_tiny_weights(size, symmetric):
+    """Scales below fp16's normal range (2^-14): half a step for the value, half a step for the zero point, and the end of the range
+    when a normal scale was rounded down (15 steps of 2^-11)."""
+    w = (np.random.default_rng(3).standard_normal((256, 40)) * size).astype(np.float32)
+    w[:64, 3] = 0.0
+    codes, scales, zeros = decode.quantize_w4(w, 64, symmetric)
+    back = D.w4_weights(codes, scales, zeros, 64, 256)
+    step = np.repeat(scales.astype(np.float64), 64, 1).T
+    assert np.all(np.abs(back - w) <= step * (1.0 + 15 * 2.0 ** -11))
+    assert scales.dtype == np.float16 and scales.flags.c_contiguous
+    assert scales[3, 0] == 0 and np.all(back[:64, 3] == 0) and (np.delete(scales.reshape(-1), 12) > 0).all()
