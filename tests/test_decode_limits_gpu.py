@@ -270,3 +270,45 @@ def test_cache_made_while_torchs_stream_is_busy(gpu_lib):
     torch.cuda.synchronize()
     assert cache.lens.tolist() == [3, 0, 2] and cache.pool[:3].tolist() == [2, 6, 0]
     assert cache.slots.tolist() == [0, 1, 2, 16, 17, -1, -1, -1]
+
+
+# ---- the accuracy of the kernel for few rows ----------------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("nq,max_q", [(1, 1), (12, 12), (40, 30)])
+def test_attention_of_few_rows_is_off_by_its_outputs_rounding_only(gpu_lib, fmt, dh, nq, max_q):
+    """Exact scores as above, without the offset. The weights go in as fp16 and the rest of that rounding (2^-22 of each, 2^-25 of
+    the largest where the rest is below the normal range), so next to the output's half step only fp32 terms are left. Weights
+    that are only rounded to fp16, planted in the oracle, are outside of the bound."""
+    rng = np.random.default_rng(dh + nq)
+    H, heads, page, n = 4, 2, 16, 60
+    pool = Pool(4, heads, page, dh, fmt, 7)
+    pool.codes[0] = D.encode(rng.integers(-3, 4, pool.shape).astype(np.float64), fmt)
+    pool.scales = [np.full((4, heads), 2.0 ** -5, np.float32), np.full((4, heads), 2.0 ** -6, np.float32)]
+    pool.raw.copy_(torch.from_numpy(np.stack(pool.codes).reshape(-1)))
+    for i in range(2):
+        pool.dev_scales[i].copy_(torch.from_numpy(pool.scales[i]))
+    q = rng.integers(-2, 3, (nq, H * dh)).astype(np.float16)
+    scale, table = 2.0, np.arange(4)[None]
+    dq, do = torch.from_numpy(q).to(DEV), torch.zeros((nq, H * dh), dtype=torch.float16, device=DEV)
+    ws, d = torch.zeros(L.KV8_WS_BYTES, dtype=torch.uint8, device=DEV), (_i32(table), _i32([n]), _i32([0, nq]))
+    assert gpu_lib.lib.sh_cuda_attention_kv8(_p(dq), _p(do), pool.handle, _p(d[0]), 4, _p(d[1]), _p(d[2]), 1, nq, max_q, H, H * dh,
+                                             H * dh, scale, _p(ws), ws.numel()) == 0
+    gpu_lib.check()
+    want, mean_abs, _, _ = D.attention_kv8(q, *pool.codes, *pool.scales, table, [n], [0, nq], H, scale, fmt)
+    # as in _offset_case, with the weights' rounding as said above
+    E = scale * 1.4427 * 6 * dh / 32 + 6
+    v = D.decode(pool.codes[1], fmt) * 2.0 ** -6
+    tol = 2.0 ** -11 * np.abs(want) + 2.0 ** -25 + n * 2.0 ** -25 * np.abs(v).max() \
+        + (2.0 ** -22 + 4 * 2.0 ** -24 * E + 2.0 ** -21 + 2 * n * 2.0 ** -24) * 1.01 * mean_abs
+    err = np.abs(_np(do).astype(np.float64) - want)
+    assert (err <= tol).all(), float((err / tol).max())
+    planted = np.zeros_like(want)
+    k = D.decode(pool.codes[0], fmt) * 2.0 ** -5
+    for i in range(nq):
+        for h in range(H):
+            keys = k[:, h // 2].reshape(-1, dh)[:n - nq + i + 1]
+            x = scale * (keys @ q[i, h * dh:(h + 1) * dh].astype(np.float64))
+            w = np.exp(x - x.max())
+            planted[i, h * dh:(h + 1) * dh] = w.astype(np.float16).astype(np.float64) @ v[:, h // 2].reshape(-1, dh)[:len(keys)] / w.sum()
+    assert (np.abs(planted.astype(np.float16).astype(np.float64) - want) > tol).any()
