@@ -176,10 +176,12 @@ int sh_cuda_kv8_append(const sh_cuda_kv8_t *cache, uint64_t k, uint64_t v, uint3
  * is a query of request r, which has lens[r] tokens in the cache, these n last, and attends its tokens
  * j <= lens[r] - n + i; query head h reads head h / (H / heads) of the cache. o = softmax(scale q k^T) v in the rows of q,
  * fp16 (leading dims ldq, ldo); a row without any token gives zeros, an infinity or a NaN in a row of q NaN in its head
- * (where the row has a token); rows of o outside [q_start[0], q_start[R]) and past T are left as they were. One token per
- * request, a few drafted ones, and whole prompt chunks are all
- * served, in any mixture. q holds T rows; max_q, the most rows of one request, only picks the kernel (a wrong value
- * costs time). ws: ws_bytes >= SH_CUDA_KV8_WS_BYTES of device memory, 16-byte aligned, zeroed once before its first use,
+ * (where the row has a token); rows of o outside [q_start[0], q_start[R]) and past T are left as they were. The rows of a
+ * request that was put off are not in the cache: they attend its tokens as if they were its last ones, and their outputs are to
+ * be ignored. One token per request, a few drafted ones, and whole prompt chunks are all served, in any mixture. q holds T rows;
+ * max_q, the most rows of one request, picks the kernel for all of them: a wrong value costs time. With max_q * H / heads > 64
+ * the softmax weights are rounded to fp16 (2^-11 of each, next to the same rounding of the output), else only the output is,
+ * so a row's last bits depend on the side that max_q is on. ws: ws_bytes >= SH_CUDA_KV8_WS_BYTES of device memory, 16-byte aligned, zeroed once before its first use,
  * for the calls of one stream at a time (a graph that may run beside other calls has its own). A table entry outside the
  * cache, or a length past ld_table * page, raises the device error word (2) and those tokens are left out. T * H < 2^31 and
  * T + ld_table * page <= 2^31 - 2^14. Returns 0, -1, or -3 for fmt. */

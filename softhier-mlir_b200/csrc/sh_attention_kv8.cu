@@ -732,7 +732,9 @@ __global__ void __launch_bounds__(NW * 32, (NT == 1 ? 16 : DH == 64 ? 12 : 8) / 
 //                 thread per row a block took 5000 cycles.
 // The scales of 16 tokens are one multiply-add per 16 scores for the maximum, one per score (x = ks s + log2 vs) and one per
 // 16 weights. A block is 2048 cycles of tensor work at its peak rate and as many of the special-function unit's (32768
-// exponentials); 32 matrix instructions of about 100 cycles each are what it cannot go below in this shape.
+// exponentials). It takes about 4800: 32 matrix instructions of about 100 cycles each, where the peak rate is 64, and what of the
+// softmax they do not cover, as a tile has one buffer for its scores. 4 x 512 rows over up to 8192 tokens: 182 us. The compiler
+// reports about 530 bytes of spilled registers at the 80 that all warps start with.
 // ================================================================================================================
 constexpr uint32_t kTlRows = 128, kTlKeys = 128, kTlItem = 256, kTlThreads = 768, kTlStages = 2;
 constexpr uint32_t kTlRegs = 96, kTlRegsOther = 48;      // 512 x 96 + 256 x 48 = 768 x 80, what the block starts with
@@ -1430,13 +1432,15 @@ int sh_cuda_attention_kv8(uint64_t q, uint64_t o, const sh_cuda_kv8_t *c, uint64
     }
     cudaError_t e;
     // Eight warps per CTA (two CTAs per SM) where items are fewer than SMs and many CTAs share one: half as many partial sums
-    // to join (131072 tokens of one request 56 us, 63 us with four). Four warps (four CTAs) where a CTA walks several items:
-    // the others go on while one ends an item (64 requests of up to 8192 tokens 115 us, 123 us with eight).
+    // to join. Four warps (four CTAs) where a CTA walks several items: the others go on while one ends an item. 32 heads over 8
+    // of 128, eight warps beside four: 131072 tokens of one request (8 items) 57 us and 64; up to 8192 tokens of 4 requests 19.5
+    // and 21.7, of 8 (64 items) 27.7 and 28.6, of 16 (128) 40.5 and 40.3, of 19 (152) 48.8 and 43.9, of 64 123 and 115.
     const bool few = (uint64_t)R * c->heads < (uint64_t)sms;
 #define SH_KV8(dh, nt, n) \
     (fp8 ? launch_rows<dh, nt, n, true>(a, mk, mv, sms, s.stream) : launch_rows<dh, nt, n, false>(a, mk, mv, sms, s.stream))
-    // 64 rows are four tiles of the kernel above: 16 requests of 7 drafts (28 rows) 77 us there, 128 us here; 4 of 64 (256 rows)
-    // 126 us there, 73 us here.
+    // The kernel above takes a tile of 16 rows after the other, this one 256 at once. 16 requests of up to 8192 tokens, heads of 128:
+    // 48 rows 106 us there and 127 here, 64 rows 136 and 128, 96 rows 179 and 131; 32 of up to 4000, heads of 64: 60 rows 56 and
+    // 66, 72 rows 70 and 66; 4 of up to 8192: 96 rows 59 and 63, 128 rows 75 and 71; a single one is level from about 200 rows on.
     if (tall) {
         a.flip = scale < 0.f ? 0x80008000u : 0u;
         a.sl2 = fabsf(a.sl2);

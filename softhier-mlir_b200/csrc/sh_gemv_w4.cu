@@ -12,8 +12,9 @@
 //          base-256 digits. The codes are int8 operands as they are (3 instructions per 8), the digits of X are six of the
 //          instruction's eight columns, of which a single row would leave seven empty, and the int32 sums of a group are
 //          exact. The zero point enters as -zero sum(digits). A 16 x 128 step takes 4 matrix instructions and 24 others, not
-//          8 and 72, but the digits take longer to lay out, so that it pays from about three tiles per SM on
-//          (49152 x 4096: 23.9 us, 30 us in fp16; 4096 x 4096: 5.6 us, 4.8 us in fp16).
+//          8 and 72, but the digits take longer to lay out, so that it pays from about three tiles per SM on (K 4096, group
+//          128, beside fp16: 2 tiles 6.1 and 5.5 us, 3 tiles 7.5 and 7.0, 3.5 tiles 7.9 and 8.2, 6 tiles 10.6 and 11.5, 49152
+//          columns 23.9 and 30; K 2048 and 8192 cross between 3 and 4 tiles as well).
 //          Infinities and NaN have no digits; outputs of such a row get those terms one by one.
 //
 // One CTA per SM: X is laid out in shared memory once, then groups of 8 warps walk tiles of 16 columns of W, each warp an
@@ -567,6 +568,8 @@ cudaError_t w4_try(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bo
     const uint32_t tiles = (a.N + 15) / 16, units = (a.K + kUnit - 1) / kUnit;
     uint32_t s = 1, room, iters;
     size_t smem;
+    // Scales copied whole, the tile's before they are needed: 16 rows of 14336 x 4096, group 128, 19.4 us, 21.1 read where they lie.
+    // At long K and group 128 their room costs X further pieces: 8 rows of 8192 x 28672 110 us, 63 without.
     // K parts over a cluster while the columns alone leave SMs idle and every warp keeps a step, or until X fits
     a.staged = (((uint64_t)a.scales | (uint64_t)a.zeros) & 15) == 0 && a.K % kUnit == 0 && a.K / G * 96 <= kMaxScales / NG;
     auto kernel = a.zeros ? k_gemv_w4<G, INT, NT, NG, D, true> : k_gemv_w4<G, INT, NT, NG, D, false>;
@@ -599,8 +602,8 @@ cudaError_t w4_try(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bo
     return cudaLaunchKernelEx(&cfg, kernel, mw, a, s, tiles, iters);
 }
 
-// Rows of X go in one piece, or in pieces of at most 16 and fewer when they do not fit beside each other. A second piece finds
-// the weights in L2 unless they are larger than that.
+// Rows of X go in one piece, or in pieces of at most 16 and fewer when they do not fit beside each other (eight for 32
+// rows of 8192 x 28672 in groups of 128). A second piece finds the weights in L2 unless they are larger than that.
 template <int G>
 cudaError_t w4_run(W4Args a, const CUtensorMap &mw, int sms, cudaStream_t st, bool &fits) {
     cudaError_t e = cudaSuccess;

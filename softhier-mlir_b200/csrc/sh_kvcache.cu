@@ -208,7 +208,9 @@ __global__ void __launch_bounds__(kTabThreads) k_kv_tables(TablesArgs a) {
 // runs of one page from the slots, max |x| per run (rows read once from HBM), the new scale, codes (rows still in
 // registers, or again from L2 when there are more than a batch), older codes of pages whose scale grew. DH / 8 lanes hold a
 // row, 16 bytes each.
-// Bound by HBM for prompts (6 bytes per element) and by latency for single tokens.
+// Bound by latency for single tokens. Prompts (6 bytes per element; 4 x 2048 tokens of 8 heads of 128, e4m3, 12.4 us where the
+// bytes take 4.2) issue 58 % of the time: each of the 2 heads CTAs of a chunk finds its window, runs and minima anew, behind six
+// barriers.
 // ================================================================================================================
 constexpr uint32_t kAppThreads = 256, kAppWin = 256 + 1;
 
@@ -226,8 +228,9 @@ struct AppendArgs {
 // the next fp32 value with 8 significant bits, for x >= 0
 __device__ __forceinline__ float up8(float x) { return __uint_as_float((__float_as_uint(x) + 0xFFFFu) & ~0xFFFFu); }
 
-// x / s, correctly rounded, from r = 1 / s (correctly rounded): the remainder is exact, so a quotient that is representable
-// (a border between two codes, which has at most 9 bits) comes out as it is. No operand here is near over- or underflow.
+// x / s from r = 1 / s (correctly rounded) and one correction by the exact remainder, Markstein's method: a quotient that is
+// representable (a border between two codes, which has at most 9 bits) comes out as it is, and the scale's 8 bits keep all others
+// further from a border than this is off. No operand here is near over- or underflow.
 __device__ __forceinline__ float divide(float x, float s, float r) {
     const float q = x * r;
     return fmaf(fmaf(-q, s, x), r, q);
