@@ -7,7 +7,9 @@
 // (int8 and e4m3 are exact in fp16) are the operands of the second product. The first product is exact up to its
 // fp32 sums. The sum of the weights is taken in fp32; for the second product they are fp16 operands, in the kernel for few
 // rows with the rest of that rounding as a second operand (the outputs' own rounding is then all there is; it costs 5 of the
-// 115 us of a large batch), in the one for many rows without it (2^-11 relative, as the outputs' own).
+// 115 us of a large batch), in the one for many rows without it: each weight is off by up to 2^-11 of itself, as the output is by
+// its own rounding. Error against 64 bits 2.9e-4, 2.1e-4 with the rests, which there cost half as many products again (4 x 512 rows
+// over up to 8192 tokens 218 us, 182 without). A caller who wants the rests passes a max_q of 1.
 #include <math.h>
 
 #include "sh_kv8.cuh"

@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(kTabThreads) k_kv_tables(TablesArgs a) {
 // registers, or again from L2 when there are more than a batch), older codes of pages whose scale grew. DH / 8 lanes hold a
 // row, 16 bytes each.
 // Bound by latency for single tokens. Prompts (6 bytes per element; 4 x 2048 tokens of 8 heads of 128, e4m3, 12.4 us where the
-// bytes take 4.2) issue 58 % of the time: each of the 2 heads CTAs of a chunk finds its window, runs and minima anew, behind six
+// bytes take 4.2) issue 57 % of the time: each of the 2 heads CTAs of a chunk finds its window, runs and minima anew, behind six
 // barriers.
 // ================================================================================================================
 constexpr uint32_t kAppThreads = 256, kAppWin = 256 + 1;
